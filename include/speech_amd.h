@@ -552,6 +552,81 @@ ctcStatus_t sa_softmax_xent(const float* logits, const long long* targets, float
                             float* dlogits, long rows, int K, void* stream);
 ctcStatus_t sa_argmax_rows(const float* x, long long* out, long rows, int K, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * 9. Output rows: a row is the V logits of one token (a CTC frame, a decoder step).  Logits are SA_F32, SA_BF16 or SA_F16 with
+ *    a last stride of one; every sum, maximum and penalty is held in 32 bits and a result is rounded to the logits' type once.
+ *    Nothing here waits for the stream or keeps state; results do not depend on timing (integer atomics only).
+ *
+ *    Constraints on the next token of a batch of requests, applied in this order to row b, token v, where c is how often v stands
+ *    in the first lengths[b] entries of history row b (entries outside [0, V) count nowhere):
+ *        c > 0:  x = x > 0 ? x / repetition : x * repetition;   x = (x - c * frequency) - presence
+ *        x += the value of the LAST entry of bias row b whose id is v (ids outside [0, V) are skipped)
+ *        x = -inf unless bit v of the request's mask row is set (word v / 32, bit v % 32, least significant first)
+ *    Each of them is optional (null / 0 / neutral).  repetition, presence, frequency: one value per row, or null and the
+ *    *_all value for every row.  The mask has n_states rows of mask_ld words and request b reads row states[b]; a state outside
+ *    [0, n_states) leaves the request unmasked; states == NULL: request b reads row b (n_states >= rows).
+ *
+ *    sa_logits_constrain writes the constrained logits (y may be x).  sa_logits_pick writes d_tokens[b] = the first index of
+ *    the row's maximum (NaN counts as the largest value; -1 when the mask leaves nothing, every value being -inf) and
+ *    d_logp[b] = its log-probability under the constrained row (-inf with -1).  No logits are written.
+ * ----------------------------------------------------------------------------------------------------------------*/
+#define SA_F32 0
+#define SA_BF16 1
+#define SA_F16 2
+#define SA_VOCAB_MAX 1048576 /* V of every operator of this section */
+#define SA_LIST_MAX 65535    /* history_len and n_bias */
+#define SA_TOP_MAX 128       /* k */
+
+typedef struct {
+    const long long* history; /* (rows, history_len) int64, rows history_ld apart, or NULL */
+    long history_ld;
+    int history_len;
+    const int* lengths; /* (rows), clamped to [0, history_len]; NULL: history_len for every row */
+    const float* repetition;
+    const float* presence;
+    const float* frequency;
+    float repetition_all, presence_all, frequency_all; /* 1, 0, 0: neutral */
+    const long long* bias_ids;                         /* (rows, n_bias), rows bias_ld apart, or NULL */
+    const float* bias_values;                          /* the same layout */
+    long bias_ld;
+    int n_bias;
+    const unsigned* mask; /* (n_states, >= ceil(V / 32)) words, or NULL */
+    long mask_ld;
+    int n_states;
+    const int* states; /* (rows) or NULL */
+} saConstraints;
+
+ctcStatus_t sa_logits_constrain(const void* x, long ldx, int dtype, void* y, long ldy, int rows, int V,
+                                const saConstraints* c, void* stream);
+size_t sa_logits_pick_workspace_bytes(int rows, int V);
+ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int rows, int V, const saConstraints* c,
+                           long long* d_tokens, float* d_logp, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The k largest logits of every row (k <= V, k <= SA_TOP_MAX) in descending order, ties to the lowest index, NaN above
+ * everything: values (rows, k) float, ids (rows, k) int64, and rest[row] = log sum exp(x_v / temperature) over the OTHER V - k
+ * tokens (-inf when there are none) -- what a distillation loss needs of a teacher's row.
+ * Row r starts at x + (r / n_inner) * ld_outer + (r % n_inner) * ld_inner. */
+size_t sa_top_logits_workspace_bytes(long rows, int V, int k, int dtype);
+ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner, int n_inner, int dtype, long rows, int V, int k,
+                          float temperature, float* values, long long* ids, float* rest, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's top logits.  Row i: the teacher's k entries (ids (rows, k), values (rows, k); an id outside
+ * [0, V) is absent; the same id may stand twice) and, when rest != NULL, the log-sum-exp of its other tokens at this
+ * temperature; q = softmax over [values / temperature, rest], p = softmax(x / temperature), p_rest = the sum of p over the tokens
+ * that are not in the list.
+ *     soft = sum_j q_j (log q_j - log p_id(j))  [+ q_rest (log q_rest - log p_rest)]     (0 for a row without entries)
+ *     hard = log sum exp(x) - x[target]                                    (0 for a target outside [0, V), or targets NULL)
+ *     loss_rows[i] = scale * weights[i] * (alpha * temperature^2 * soft + (1 - alpha) * hard);   *loss = their sum
+ * A row of weight 0 is not read: its loss and its gradient are 0 whatever it holds.  weights NULL: 1.
+ * dx (the layout of x, or NULL) = the gradient of *loss with respect to x, times *d_factor when d_factor != NULL.
+ * loss == NULL: only the gradient; then skip_unit != 0 leaves dx untouched when *d_factor is 1 (dx holds it already).
+ * loss_rows (rows floats) is written whenever loss is. */
+ctcStatus_t sa_distill_loss(const void* x, void* dx, long ld_outer, long ld_inner, int n_inner, int dtype, long rows,
+                            int V, const float* values, const long long* ids, const float* rest, int k,
+                            const long long* targets, const float* weights, float temperature, float alpha, float scale,
+                            const float* d_factor, int skip_unit, float* loss_rows, float* loss, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

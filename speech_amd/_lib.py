@@ -27,6 +27,14 @@ class ctcOptions(ctypes.Structure):
     _fields_ = [("loc", c_int), ("u", _U), ("blank_label", c_int)]
 
 
+class saConstraints(ctypes.Structure):
+    _fields_ = [("history", c_void_p), ("history_ld", c_long), ("history_len", c_int), ("lengths", c_void_p),
+                ("repetition", c_void_p), ("presence", c_void_p), ("frequency", c_void_p), ("repetition_all", c_float),
+                ("presence_all", c_float), ("frequency_all", c_float), ("bias_ids", c_void_p), ("bias_values", c_void_p),
+                ("bias_ld", c_long), ("n_bias", c_int), ("mask", c_void_p), ("mask_ld", c_long), ("n_states", c_int),
+                ("states", c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/speech_amd.h declares
 SIGNATURES = {
     "get_warpctc_version": (c_int, []),
@@ -142,6 +150,17 @@ SIGNATURES = {
                                                                                                   c_void_p, c_size_t, c_void_p]),
     "sa_softmax_xent": (c_int, [c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_long, c_int, c_void_p]),
     "sa_argmax_rows": (c_int, [c_void_p, c_void_p, c_long, c_int, c_void_p]),
+    "sa_logits_constrain": (c_int, [c_void_p, c_long, c_int, c_void_p, c_long, c_int, c_int,
+                                    ctypes.POINTER(saConstraints), c_void_p]),
+    "sa_logits_pick_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "sa_logits_pick": (c_int, [c_void_p, c_long, c_int, c_int, c_int, ctypes.POINTER(saConstraints), c_void_p, c_void_p,
+                               c_void_p, c_size_t, c_void_p]),
+    "sa_top_logits_workspace_bytes": (c_size_t, [c_long, c_int, c_int, c_int]),
+    "sa_top_logits": (c_int, [c_void_p, c_long, c_long, c_int, c_int, c_long, c_int, c_int, c_float, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sa_distill_loss": (c_int, [c_void_p, c_void_p, c_long, c_long, c_int, c_int, c_long, c_int, c_void_p, c_void_p, c_void_p,
+                                c_int, c_void_p, c_void_p, c_float, c_float, c_float, c_void_p, c_int, c_void_p, c_void_p,
+                                c_void_p]),
     "sa_sgd_workspace_bytes": (c_size_t, [c_size_t]),
     "sa_clip_sgd_step": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_float, c_float, c_float, c_float, c_void_p,
                                  c_void_p, c_void_p, c_size_t, c_void_p]),
