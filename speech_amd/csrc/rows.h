@@ -70,3 +70,47 @@ __device__ __forceinline__ float sa_unorder(unsigned k) {  // the inverse
 __device__ __forceinline__ unsigned long long sa_rank_key(float x, int i) {
     return ((unsigned long long)sa_order(x) << 32) | (unsigned)~(unsigned)i;
 }
+
+// ---- a row as vectors of 16 bytes ------------------------------------------------------------------------------------------
+// Rows start anywhere (odd V, views): vector q of a row covers its elements [q VEC - lead, q VEC - lead + VEC), where `lead` is how
+// many elements the row starts behind a 16-byte boundary.  Every whole vector is then one aligned 16-byte access and only a row's
+// first and last vector can be partial; those go element by element, so nothing outside the row is touched.
+template <typename T> struct SaVec { static constexpr int N = 16 / (int)sizeof(T); };
+template <typename T> __device__ __forceinline__ unsigned sa_fill_word();  // -inf in every element
+template <> __device__ __forceinline__ unsigned sa_fill_word<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ unsigned sa_fill_word<SaBf16>() { return 0xff80ff80u; }
+template <> __device__ __forceinline__ unsigned sa_fill_word<SaF16>() { return 0xfc00fc00u; }
+
+template <typename T> __device__ __forceinline__ int sa_lead(const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); }
+
+template <typename T> __device__ __forceinline__ float sa_element(const uint4& q, int e);
+template <> __device__ __forceinline__ float sa_element<float>(const uint4& q, int e) {
+    return __builtin_bit_cast(float, e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w);
+}
+template <> __device__ __forceinline__ float sa_element<SaBf16>(const uint4& q, int e) {
+    const unsigned w = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
+    return __builtin_bit_cast(float, e & 1 ? w & 0xffff0000u : w << 16);
+}
+template <> __device__ __forceinline__ float sa_element<SaF16>(const uint4& q, int e) {
+    const unsigned w = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
+    return (float)__builtin_bit_cast(_Float16, (sa_u16)(e & 1 ? w >> 16 : w));
+}
+
+// the vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V)
+template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* __restrict__ row, int v0, int V) {
+    if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
+    const unsigned f = sa_fill_word<T>();
+    unsigned w[4] = {f, f, f, f};
+#pragma unroll
+    for (int e = 0; e < SaVec<T>::N; ++e) {
+        const int v = v0 + e;
+        if (v < 0 || v >= V) continue;
+        if constexpr (sizeof(T) == 4) {
+            w[e] = __builtin_bit_cast(unsigned, row[v]);
+        } else {
+            const unsigned h = __builtin_bit_cast(sa_u16, row[v]);
+            w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | (h << 16) : (w[e >> 1] & 0xffff0000u) | h;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
