@@ -5,11 +5,15 @@
 // with the type's lowest value stays finite (a fused x c - m c would leave the rounding error of m c, which is huge there).
 // The listed tokens and the rest have maxima and sums of their own: p_rest is a sum of its own terms and no difference from 1, and
 // it does not vanish when the rest lies far below the list.
+//
+// A workgroup per row.  The row is read once, as 16-byte vectors, into registers (what is beyond NT * NV vectors is read a second
+// time); each thread sums relative to its own maximum, the waves' results are joined in one exchange through LDS, and the
+// gradient is formed from the registers.  Listed tokens are marked in a bitmap in LDS and taken out of the sums where the rest is
+// a class of its own; their gradients replace what the row-wide formula wrote.  The teacher's side of a row is k <= 128
+// numbers: the first wave does it, two to a lane, while the others sum.
 #include "rows.h"
 
 namespace {
-
-constexpr int kDisThreads = 256, kDisWaves = kDisThreads / 64;
 
 struct DisArgs {
     const float* values;
@@ -24,120 +28,255 @@ struct DisArgs {
     float* loss_rows;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kDisThreads) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, DisArgs A) {
-    extern __shared__ unsigned bitmap[];  // V bits: the token is in the list
-    __shared__ float scratch[kDisWaves];
+struct DisSum { float m, s, h; };  // maximum, sum of exp((x - m) / T), sum of exp(x - m)
+
+// a maximum that can be subtracted: -inf (nothing there) counts as 0, and every exp2((-inf - 0) c) is 0
+__device__ __forceinline__ float dis_base(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// REST: the rest is a class, and the list is taken out of the sums.  TWO: the sums at temperatures T and 1 differ and both are wanted.
+template <typename T, int NT, int NV, bool REST, bool TWO>
+__global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, DisArgs A) {
+    constexpr int VEC = SaVec<T>::N, NW = NT / 64;
+    extern __shared__ unsigned bitmap[];  // a bit per element of the row's vectors: the token is in the list
+    __shared__ DisSum waves[NW];
     __shared__ int ids[SA_TOP_MAX];
-    __shared__ float q[SA_TOP_MAX];
+    __shared__ float qs[SA_TOP_MAX];
+    __shared__ float list[4];  // what the first wave found: maximum and sums over the list, q of the rest
+    __shared__ int soft_row;
     const long row = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     float f = A.scale;
     if (A.factor) {
-        if (A.skip_unit && *A.factor == 1.0f) return;
-        f *= *A.factor;
+        const float g = *A.factor;
+        if (A.skip_unit && g == 1.0f) return;
+        f *= g;
     }
     const float w = A.weights ? A.weights[row] : 1.0f;
     const T* xr = x + at.at(row);
     T* dr = dx ? dx + at.at(row) : nullptr;
+    const int lead = sa_lead(xr);
+    const bool aligned = dr && sa_lead(dr) == lead;
+    const int nq = (V + lead + VEC - 1) / VEC;
     if (w == 0.0f) {  // nothing of the row is read: it may hold anything
+        const float zero[VEC] = {};
         if (dr)
-            for (int v = tid; v < V; v += kDisThreads) dr[v] = sa_narrow<T>(0.0f);
+            for (int q = tid; q < nq; q += NT) sa_store_vec<T>(dr, q * VEC - lead, V, zero, aligned);
         if (A.loss_rows && tid == 0) A.loss_rows[row] = 0.0f;
         return;
     }
     f *= w;
 
-    // the teacher: log q and q of the list and of the rest
-    for (int i = tid; i < (V + 31) / 32; i += kDisThreads) bitmap[i] = 0;
-    __syncthreads();
-    int id = -1;
-    float a = -INFINITY;
-    if (tid < A.k) {
-        const long long t = A.ids[row * A.k + tid];
-        if (t >= 0 && t < V) {
-            id = (int)t;
-            a = A.values[row * A.k + tid] / A.temperature;
-            atomicOr(&bitmap[id >> 5], 1u << (id & 31));
-        }
-        ids[tid] = id;
-    }
-    const bool resting = A.rest != nullptr;
-    const float ar = resting ? A.rest[row] : -INFINITY;
-    const float am = fmaxf(sa_block_max<kDisWaves>(a, scratch), ar);
-    const bool soft = am > -INFINITY && A.alpha > 0.0f;
-    const float e = soft ? sa_exp2((a - am) * SA_LOG2E) : 0.0f, er = soft && resting ? sa_exp2((ar - am) * SA_LOG2E) : 0.0f;
-    const float total = sa_block_sum<kDisWaves>(e, scratch) + er;
-    const float lt = logf(total), qj = soft ? e / total : 0.0f, qr = soft ? er / total : 0.0f;
-    if (tid < A.k) q[tid] = qj;
-    __syncthreads();
-
-    // the student: maxima and sums over the list (first occurrence of an id) and over the others
-    bool first = id >= 0;
-    float qsum = 0.0f;  // over the entries of the same id
-    if (id >= 0)
-        for (int j = 0; j < A.k; ++j)
-            if (ids[j] == id) {
-                if (j < tid) first = false;
-                qsum += q[j];
+    uint4 raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, (i * NT + tid) * VEC - lead, V);
+    // the list: marked in the bitmap by the first wave, two entries a lane
+    int id[2] = {-1, -1};
+    float a[2] = {-INFINITY, -INFINITY}, xv[2] = {-INFINITY, -INFINITY};
+    for (int i = tid; i < (nq * VEC + 31) / 32; i += NT) bitmap[i] = 0;
+    if (tid < 64) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int j = lane + 64 * i;
+            if (j >= A.k) continue;
+            const long long t = A.ids[row * A.k + j];
+            if (t >= 0 && t < V) {
+                id[i] = (int)t;
+                a[i] = A.values[row * A.k + j] / A.temperature;
+                xv[i] = sa_widen(xr[t]);
             }
-    const float c = SA_LOG2E / A.temperature;
-    const float xv = id >= 0 ? sa_widen(xr[id]) : -INFINITY;
-    float mr = -INFINITY;
-    for (int v = tid; v < V; v += kDisThreads)
-        if (!((bitmap[v >> 5] >> (v & 31)) & 1u)) mr = fmaxf(mr, sa_widen(xr[v]));
-    mr = sa_block_max<kDisWaves>(mr, scratch);
-    const float mt = sa_block_max<kDisWaves>(first ? xv : -INFINITY, scratch);
-    const float m = fmaxf(mr, mt);
-    const bool hard_on = A.alpha < 1.0f && A.targets;
-    float sr = 0.0f, hr = 0.0f;
-    for (int v = tid; v < V; v += kDisThreads)
-        if (!((bitmap[v >> 5] >> (v & 31)) & 1u)) {
-            const float d = sa_widen(xr[v]) - mr;
-            sr += sa_exp2(d * c);
-            hr += sa_exp2(d * SA_LOG2E);
         }
-    if (mr == -INFINITY) sr = hr = 0.0f;
-    sr = sa_block_sum<kDisWaves>(sr, scratch);
-    hr = sa_block_sum<kDisWaves>(hr, scratch);
-    const float st = sa_block_sum<kDisWaves>(first ? sa_exp2((xv - mt) * c) : 0.0f, scratch);
-    const float ht = sa_block_sum<kDisWaves>(first ? sa_exp2((xv - mt) * SA_LOG2E) : 0.0f, scratch);
-    // over all tokens, relative to m
-    const float S = (mr > -INFINITY ? sr * sa_exp2((mr - m) * c) : 0.0f) + (mt > -INFINITY ? st * sa_exp2((mt - m) * c) : 0.0f);
-    const float H = (mr > -INFINITY ? hr * sa_exp2((mr - m) * SA_LOG2E) : 0.0f) +
-                    (mt > -INFINITY ? ht * sa_exp2((mt - m) * SA_LOG2E) : 0.0f);
-    const float lS = logf(S), lH = logf(H);
-    const float logpr = (mr - m) / A.temperature + logf(sr) - lS;
+    }
+    __syncthreads();
+    bool twice = false;  // some id stands in the list more than once
+    if (tid < 64) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int j = lane + 64 * i, p = id[i] + lead;
+            if (id[i] >= 0) twice |= (atomicOr(&bitmap[p >> 5], 1u << (p & 31)) >> (p & 31)) & 1u;
+            if (j < A.k) ids[j] = id[i];
+        }
+        twice = __any(twice);
+    }
+    __syncthreads();
 
-    const long long target = hard_on ? A.targets[row] : -1;
+    // the teacher: q of the list and of the rest; the student's sums over the list (each id once)
+    const float c = SA_LOG2E / A.temperature;
+    bool first[2] = {false, false}, soft = false;
+    float q[2], qsum[2], am = 0.0f, lt = 0.0f, qr = 0.0f, ar = -INFINITY;
+    if (tid < 64) {
+        if (REST) ar = A.rest[row];
+        am = fmaxf(sa_wave_max(fmaxf(a[0], a[1])), ar);
+        soft = am > -INFINITY && A.alpha > 0.0f;
+        const float e0 = soft ? sa_exp2((a[0] - am) * SA_LOG2E) : 0.0f, e1 = soft ? sa_exp2((a[1] - am) * SA_LOG2E) : 0.0f;
+        const float er = soft && REST ? sa_exp2((ar - am) * SA_LOG2E) : 0.0f;
+        const float total = sa_wave_sum(e0 + e1) + er;
+        lt = logf(total);
+        q[0] = soft ? e0 / total : 0.0f;
+        q[1] = soft ? e1 / total : 0.0f;
+        qr = soft ? er / total : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            first[i] = id[i] >= 0;
+            qsum[i] = q[i];
+            if (lane + 64 * i < A.k) qs[lane + 64 * i] = q[i];
+        }
+        if (twice) {  // in the order of the list, whoever marked the bit
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (id[i] < 0) continue;
+                qsum[i] = 0.0f;
+                for (int j = 0; j < A.k; ++j)
+                    if (ids[j] == id[i]) {
+                        if (j < lane + 64 * i) first[i] = false;
+                        qsum[i] += qs[j];
+                    }
+            }
+        }
+        if (REST) {
+            const float y0 = first[0] ? xv[0] : -INFINITY, y1 = first[1] ? xv[1] : -INFINITY;
+            const float mt = sa_wave_max(fmaxf(y0, y1)), b = dis_base(mt);
+            const float st = sa_wave_sum(sa_exp2((y0 - b) * c) + sa_exp2((y1 - b) * c));
+            const float ht = TWO ? sa_wave_sum(sa_exp2((y0 - b) * SA_LOG2E) + sa_exp2((y1 - b) * SA_LOG2E)) : st;
+            if (lane == 0) { list[0] = mt; list[1] = st; list[2] = ht; }
+        }
+        if (lane == 0) { list[3] = qr; soft_row = soft; }
+    }
+
+    // the student: all tokens, or those that are not in the list
+    DisSum d{-INFINITY, 0.0f, 0.0f};
+    auto marks = [&](int v) { return (bitmap[v >> 5] >> (v & 31)) & ((1u << VEC) - 1u); };
+    auto drop = [&](uint4& r, int q0) {
+        const unsigned bits = marks(q0 * VEC);
+        if (bits) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if ((bits >> e) & 1u) sa_drop_element<T>(r, e);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (REST && i * NT + tid < nq) drop(raw[i], i * NT + tid);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) d.m = fmaxf(d.m, sa_element<T>(raw[i], e));
+    }
+    {
+        const float b = dis_base(d.m);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float t = sa_element<T>(raw[i], e) - b;
+                d.s += sa_exp2(t * c);
+                if (TWO) d.h += sa_exp2(t * SA_LOG2E);
+            }
+    }
+    for (int p = NV * NT + tid; p < nq; p += NT) {  // what the registers did not hold
+        uint4 r = sa_load_vec(xr, p * VEC - lead, V);
+        if (REST) drop(r, p);
+        float m = d.m;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = fmaxf(m, sa_element<T>(r, e));
+        const float b = dis_base(m), o = d.m - b;
+        d.s *= sa_exp2(o * c);
+        if (TWO) d.h *= sa_exp2(o * SA_LOG2E);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float t = sa_element<T>(r, e) - b;
+            d.s += sa_exp2(t * c);
+            if (TWO) d.h += sa_exp2(t * SA_LOG2E);
+        }
+        d.m = m;
+    }
+    {   // the wave, then the waves in their order
+        const float m = sa_wave_max_dpp(d.m), o = d.m - dis_base(m);
+        d.s = sa_wave_sum_dpp(d.s * sa_exp2(o * c));
+        d.h = TWO ? sa_wave_sum_dpp(d.h * sa_exp2(o * SA_LOG2E)) : d.s;
+        d.m = m;
+    }
+    if (lane == 0) waves[tid >> 6] = d;
+    __syncthreads();
+    float mr = waves[0].m, sr = 0.0f, hr = 0.0f;
+#pragma unroll
+    for (int i = 1; i < NW; ++i) mr = fmaxf(mr, waves[i].m);
+    const float br = dis_base(mr);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const float o = waves[i].m - br;
+        sr += waves[i].s * sa_exp2(o * c);
+        if (TWO) hr += waves[i].h * sa_exp2(o * SA_LOG2E);
+    }
+    if (!TWO) hr = sr;
+    // over all tokens, relative to m
+    float m = mr, S = sr, H = hr, pr = 1.0f, ph = 1.0f;
+    if (REST) {
+        m = fmaxf(mr, list[0]);
+        const float b = dis_base(m), t = list[0] - b, o = mr - b;
+        const float er = sa_exp2(o * c), eh = TWO ? sa_exp2(o * SA_LOG2E) : er;
+        S = sr * er + list[1] * sa_exp2(t * c);
+        H = TWO ? hr * eh + list[2] * sa_exp2(t * SA_LOG2E) : S;
+        pr = sr == 0.0f ? 0.0f : sr * er / S;   // the student's p of the rest, at T and at 1
+        ph = hr == 0.0f ? 0.0f : hr * eh / H;
+        qr = list[3];
+    }
+    soft = soft_row != 0;
+    const long long target = A.alpha < 1.0f && A.targets ? A.targets[row] : -1;
     const bool hard = target >= 0 && target < V;
-    if (A.loss_rows) {
-        float l = qj > 0.0f ? qj * ((a - am) - lt - ((xv - m) / A.temperature - lS)) : 0.0f;
-        l = sa_block_sum<kDisWaves>(l, scratch);
-        if (tid == 0) {
-            if (qr > 0.0f) l += qr * ((ar - am) - lt - logpr);
+
+    if (A.loss_rows && tid < 64) {
+        const float lS = logf(S);
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (q[i] > 0.0f) l += q[i] * ((a[i] - am) - lt - ((xv[i] - m) / A.temperature - lS));
+        l = sa_wave_sum(l);
+        if (lane == 0) {
+            if (REST && qr > 0.0f) l += qr * ((ar - am) - lt - ((mr - m) / A.temperature + logf(sr) - lS));
             float v = soft ? A.alpha * A.temperature * A.temperature * l : 0.0f;
-            if (hard) v += (1.0f - A.alpha) * (lH - (sa_widen(xr[target]) - m));
+            if (hard) v += (1.0f - A.alpha) * (logf(H) - (sa_widen(xr[target]) - m));
             A.loss_rows[row] = f * v;
         }
     }
     if (!dr) return;
     // the gradient: a row-wide formula for the tokens that are not in the list -- relative to THEIR maximum, so that nothing
-    // overflows where the list is far above them: p_v = p_rest r_v with r = softmax over the rest --, then the list
+    // overflows where the list is far above them: p_v = p_rest r_v with r = softmax over the rest --, then the list and the target
     const float cs = soft ? f * A.alpha * A.temperature : 0.0f, ch = hard ? f * (1.0f - A.alpha) : 0.0f;
-    const float pr = sr == 0.0f ? 0.0f : sr * sa_exp2((mr - m) * c) / S;
-    const float kr = sr == 0.0f ? 0.0f : cs * (pr - qr) / sr, kh = hr == 0.0f ? 0.0f : ch * sa_exp2((mr - m) * SA_LOG2E) / H;
-    const float base = mr > -INFINITY ? mr : 0.0f;
-    for (int v = tid; v < V; v += kDisThreads)
-        if (!((bitmap[v >> 5] >> (v & 31)) & 1u)) {
-            const float d = sa_widen(xr[v]) - base;
-            const float g = kr * sa_exp2(d * c) + kh * sa_exp2(d * SA_LOG2E) - (v == target ? ch : 0.0f);
-            dr[v] = sa_narrow<T>(g);
+    const bool live = cs != 0.0f || ch != 0.0f;  // (a row without a list and without a target: zeros, whatever it holds)
+    float kr = sr == 0.0f ? 0.0f : cs * (REST ? pr - qr : 1.0f) / sr, kh = hr == 0.0f ? 0.0f : ch * ph / hr;
+    if (!TWO) kr += kh;
+    auto grad = [&](uint4& r, int q0) {
+        float g[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float t = sa_element<T>(r, e) - br;
+            g[e] = kr * sa_exp2(t * c);
+            if (TWO) g[e] += kh * sa_exp2(t * SA_LOG2E);
+            if (!live) g[e] = 0.0f;
         }
-    if (first) {
-        const float d = xv - m;
-        const float g = cs * (sa_exp2(d * c) / S - qsum) + ch * sa_exp2(d * SA_LOG2E) / H - (id == target ? ch : 0.0f);
-        dr[id] = sa_narrow<T>(g);
+        sa_store_vec<T>(dr, q0 * VEC - lead, V, g, aligned);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (i * NT + tid < nq) grad(raw[i], i * NT + tid);
+    for (int p = NV * NT + tid; p < nq; p += NT) {
+        uint4 r = sa_load_vec(xr, p * VEC - lead, V);
+        grad(r, p);
+    }
+    __syncthreads();
+    if (tid < 64 && live) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (first[i]) {
+                const float t = xv[i] - m;
+                const float g = cs * (sa_exp2(t * c) / S - qsum[i]) + (hard ? ch * (sa_exp2(t * SA_LOG2E) / H - (id[i] == target ? 1.0f : 0.0f)) : 0.0f);
+                dr[id[i]] = sa_narrow<T>(g);
+            }
+        if (lane == 0 && hard && !((bitmap[(target + lead) >> 5] >> ((target + lead) & 31)) & 1u)) {
+            const float t = sa_widen(xr[target]) - br;
+            const float g = (TWO ? kr * sa_exp2(t * c) + kh * sa_exp2(t * SA_LOG2E) : kr * sa_exp2(t * c)) - ch;
+            dr[target] = sa_narrow<T>(g);
+        }
     }
 }
 
@@ -156,14 +295,34 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     }
 }
 
+template <typename T, int NT, int NV, bool REST, bool TWO>
+bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
+    const size_t smem = (size_t)((V + 2 * SaVec<T>::N + 31) / 32) * 4;
+    if (smem > 48 * 1024 && hipFuncSetAttribute((const void*)distill_kernel<T, NT, NV, REST, TWO>,
+                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+        return false;
+    hipLaunchKernelGGL((distill_kernel<T, NT, NV, REST, TWO>), dim3((unsigned)rows), dim3(NT), smem, stream, (const T*)x, (T*)dx, at, V,
+                       A);
+    return true;
+}
+
+template <typename T, int NT, int NV>
+bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
+    const bool two = A.alpha < 1.0f && A.targets && A.temperature != 1.0f;
+    if (A.rest) return two ? dis_run<T, NT, NV, true, true>(x, dx, at, rows, V, A, stream)
+                           : dis_run<T, NT, NV, true, false>(x, dx, at, rows, V, A, stream);
+    return two ? dis_run<T, NT, NV, false, true>(x, dx, at, rows, V, A, stream)
+               : dis_run<T, NT, NV, false, false>(x, dx, at, rows, V, A, stream);
+}
+
+// the smallest workgroup whose registers hold a row
 template <typename T>
 bool dis_launch(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    const size_t smem = (size_t)((V + 31) / 32) * 4;
-    if (smem > 48 * 1024 && hipFuncSetAttribute((const void*)distill_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                (int)smem) != hipSuccess)
-        return false;
-    hipLaunchKernelGGL((distill_kernel<T>), dim3((unsigned)rows), dim3(kDisThreads), smem, stream, (const T*)x, (T*)dx, at, V, A);
-    return true;
+    const int vectors = (V + 2 * SaVec<T>::N - 2) / SaVec<T>::N;
+    if (vectors <= 64 * 2) return dis_pick<T, 64, 2>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 256 * 8) return dis_pick<T, 256, 8>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 512 * 16) return dis_pick<T, 512, 16>(x, dx, at, rows, V, A, stream);
+    return dis_pick<T, 1024, 16>(x, dx, at, rows, V, A, stream);
 }
 
 }  // namespace

@@ -96,6 +96,43 @@ template <> __device__ __forceinline__ float sa_element<SaF16>(const uint4& q, i
     return (float)__builtin_bit_cast(_Float16, (sa_u16)(e & 1 ? w >> 16 : w));
 }
 
+// element e becomes -inf
+template <typename T> __device__ __forceinline__ void sa_drop_element(uint4& q, int e) {
+    constexpr int per = 4 / (int)sizeof(T);
+    unsigned* const w[4] = {&q.x, &q.y, &q.z, &q.w};
+    unsigned& u = *w[e / per];
+    if constexpr (per == 1) u = sa_fill_word<T>();
+    else u = e & 1 ? (u & 0xffffu) | (sa_fill_word<T>() & 0xffff0000u) : (u & 0xffff0000u) | (sa_fill_word<T>() & 0xffffu);
+}
+
+// eight or four results, rounded to the type
+template <typename T> __device__ __forceinline__ uint4 sa_pack(const float* g);
+template <> __device__ __forceinline__ uint4 sa_pack<float>(const float* g) {
+    return make_uint4(__builtin_bit_cast(unsigned, g[0]), __builtin_bit_cast(unsigned, g[1]), __builtin_bit_cast(unsigned, g[2]),
+                      __builtin_bit_cast(unsigned, g[3]));
+}
+template <> __device__ __forceinline__ uint4 sa_pack<SaBf16>(const float* g) {
+    return make_uint4(sa_cvt_pk_bf16(g[0], g[1]), sa_cvt_pk_bf16(g[2], g[3]), sa_cvt_pk_bf16(g[4], g[5]), sa_cvt_pk_bf16(g[6], g[7]));
+}
+template <> __device__ __forceinline__ uint4 sa_pack<SaF16>(const float* g) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = (unsigned)sa_narrow<SaF16>(g[2 * i]).v | ((unsigned)sa_narrow<SaF16>(g[2 * i + 1]).v << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// the vector whose first element is v0, into a row that starts at the same offset from a 16-byte boundary
+template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v0, int V, const float* g, bool aligned) {
+    if (aligned && v0 >= 0 && v0 + SaVec<T>::N <= V) {
+        *reinterpret_cast<uint4*>(row + v0) = sa_pack<T>(g);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < SaVec<T>::N; ++e)
+        if (v0 + e >= 0 && v0 + e < V) row[v0 + e] = sa_narrow<T>(g[e]);
+}
+
 // the vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V)
 template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* __restrict__ row, int v0, int V) {
     if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
