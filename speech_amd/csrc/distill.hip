@@ -8,7 +8,8 @@
 //
 // A workgroup per row.  The row is read once, as 16-byte vectors, into registers (what is beyond NT * NV vectors is read a second
 // time); each thread sums relative to its own maximum, the waves' results are joined in one exchange through LDS, and the
-// gradient is formed from the registers.  Listed tokens are marked in a bitmap in LDS and taken out of the sums where the rest is
+// gradient is formed from the registers: from the exponentials themselves where they fit (KEEP), one or two multiplications an
+// element, else from the logits again.  At T = 2 and T = 4 the second sum takes exp(x - m) as a power of exp((x - m) / T).  Listed tokens are marked in a bitmap in LDS and taken out of the sums where the rest is
 // a class of its own; their gradients replace what the row-wide formula wrote.  The teacher's side of a row is k <= 128
 // numbers: the first wave does it, two to a lane, while the others sum.
 #include "rows.h"
@@ -33,10 +34,13 @@ struct DisSum { float m, s, h; };  // maximum, sum of exp((x - m) / T), sum of e
 // a maximum that can be subtracted: -inf (nothing there) counts as 0, and every exp2((-inf - 0) c) is 0
 __device__ __forceinline__ float dis_base(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// REST: the rest is a class, and the list is taken out of the sums.  TWO: the sums at temperatures T and 1 differ and both are wanted.
-template <typename T, int NT, int NV, bool REST, bool TWO>
+// REST: the rest is a class, and the list is taken out of the sums.  The sum at temperature 1 beside the one at T, HARD: 0 not wanted
+// or the same; 1 by its own exponential; 2, 4 as that power of the one at T = 2, 4.
+template <typename T, int NT, int NV, bool KEEP, bool REST, int HARD>
 __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, DisArgs A) {
     constexpr int VEC = SaVec<T>::N, NW = NT / 64;
+    constexpr bool TWO = HARD != 0;
+    static_assert(!KEEP || HARD != 1, "only one exponential of an element is kept");
     extern __shared__ unsigned bitmap[];  // a bit per element of the row's vectors: the token is in the list
     __shared__ DisSum waves[NW];
     __shared__ int ids[SA_TOP_MAX];
@@ -155,22 +159,35 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
                 if ((bits >> e) & 1u) sa_drop_element<T>(r, e);
         }
     };
+    auto power = [](float e) { return HARD == 2 ? e * e : (e * e) * (e * e); };
+    // (the logits of two bytes are widened again for every use: kept as they are, they would take twice the registers)
+    auto again = [](uint4& r) {
+        if constexpr (sizeof(T) == 2 && !KEEP) asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (REST && i * NT + tid < nq) drop(raw[i], i * NT + tid);
+        if (i * NT < nq) {
+            if (REST && i * NT + tid < nq) drop(raw[i], i * NT + tid);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) d.m = fmaxf(d.m, sa_element<T>(raw[i], e));
+            for (int e = 0; e < VEC; ++e) d.m = fmaxf(d.m, sa_element<T>(raw[i], e));
+            again(raw[i]);
+        }
     }
-    {
-        const float b = dis_base(d.m);
+    const float own = d.m, bt = dis_base(own);
+    float kept[KEEP ? NV * VEC : 1];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        if (i * NT < nq) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float t = sa_element<T>(raw[i], e) - b;
-                d.s += sa_exp2(t * c);
-                if (TWO) d.h += sa_exp2(t * SA_LOG2E);
+                const float t = sa_element<T>(raw[i], e) - bt, u = sa_exp2(t * c);
+                d.s += u;
+                if (HARD == 1) d.h += sa_exp2(t * SA_LOG2E);
+                if (HARD > 1) d.h += power(u);
+                if (KEEP) kept[i * VEC + e] = u;
             }
+            again(raw[i]);
+        }
     }
     for (int p = NV * NT + tid; p < nq; p += NT) {  // what the registers did not hold
         uint4 r = sa_load_vec(xr, p * VEC - lead, V);
@@ -183,9 +200,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
         if (TWO) d.h *= sa_exp2(o * SA_LOG2E);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float t = sa_element<T>(r, e) - b;
-            d.s += sa_exp2(t * c);
-            if (TWO) d.h += sa_exp2(t * SA_LOG2E);
+            const float t = sa_element<T>(r, e) - b, u = sa_exp2(t * c);
+            d.s += u;
+            if (HARD == 1) d.h += sa_exp2(t * SA_LOG2E);
+            if (HARD > 1) d.h += power(u);
         }
         d.m = m;
     }
@@ -245,26 +263,46 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
     const bool live = cs != 0.0f || ch != 0.0f;  // (a row without a list and without a target: zeros, whatever it holds)
     float kr = sr == 0.0f ? 0.0f : cs * (REST ? pr - qr : 1.0f) / sr, kh = hr == 0.0f ? 0.0f : ch * ph / hr;
     if (!TWO) kr += kh;
+    if (!live) {
+        const float zero[VEC] = {};
+        for (int p = tid; p < nq; p += NT) sa_store_vec<T>(dr, p * VEC - lead, V, zero, aligned);
+        return;
+    }
     auto grad = [&](uint4& r, int q0) {
         float g[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float t = sa_element<T>(r, e) - br;
-            g[e] = kr * sa_exp2(t * c);
-            if (TWO) g[e] += kh * sa_exp2(t * SA_LOG2E);
-            if (!live) g[e] = 0.0f;
+            const float t = sa_element<T>(r, e) - br, u = sa_exp2(t * c);
+            g[e] = kr * u;
+            if (HARD == 1) g[e] += kh * sa_exp2(t * SA_LOG2E);
+            if (HARD > 1) g[e] += kh * power(u);
         }
         sa_store_vec<T>(dr, q0 * VEC - lead, V, g, aligned);
     };
+    // (the kept exponentials are relative to the thread's own maximum; a thread without a finite one kept zeros)
+    const float shift = own == -INFINITY ? 0.0f : sa_exp2((bt - br) * c), krt = kr * shift, kht = HARD > 1 ? kh * power(shift) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (i * NT + tid < nq) grad(raw[i], i * NT + tid);
+    for (int i = 0; i < NV; ++i) {
+        const int p = i * NT + tid;
+        if (p >= nq) continue;
+        if constexpr (KEEP) {
+            float g[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float u = kept[i * VEC + e];
+                g[e] = HARD > 1 ? krt * u + kht * power(u) : krt * u;
+            }
+            sa_store_vec<T>(dr, p * VEC - lead, V, g, aligned);
+        } else {
+            grad(raw[i], p);
+        }
+    }
     for (int p = NV * NT + tid; p < nq; p += NT) {
         uint4 r = sa_load_vec(xr, p * VEC - lead, V);
         grad(r, p);
     }
     __syncthreads();
-    if (tid < 64 && live) {
+    if (tid < 64) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (first[i]) {
@@ -295,34 +333,41 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     }
 }
 
-template <typename T, int NT, int NV, bool REST, bool TWO>
+template <typename T, int NT, int NV, bool KEEP, bool REST, int HARD>
 bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
     const size_t smem = (size_t)((V + 2 * SaVec<T>::N + 31) / 32) * 4;
-    if (smem > 48 * 1024 && hipFuncSetAttribute((const void*)distill_kernel<T, NT, NV, REST, TWO>,
-                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+    constexpr auto kernel = distill_kernel<T, NT, NV, KEEP && HARD != 1, REST, HARD>;
+    if (smem > 48 * 1024 &&
+        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
         return false;
-    hipLaunchKernelGGL((distill_kernel<T, NT, NV, REST, TWO>), dim3((unsigned)rows), dim3(NT), smem, stream, (const T*)x, (T*)dx, at, V,
-                       A);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(NT), smem, stream, (const T*)x, (T*)dx, at, V, A);
     return true;
 }
 
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool KEEP, bool REST>
+bool dis_hard(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
+    if (A.alpha == 1.0f || !A.targets || A.temperature == 1.0f) return dis_run<T, NT, NV, KEEP, REST, 0>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 2.0f) return dis_run<T, NT, NV, KEEP, REST, 2>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 4.0f) return dis_run<T, NT, NV, KEEP, REST, 4>(x, dx, at, rows, V, A, stream);
+    return dis_run<T, NT, NV, KEEP, REST, 1>(x, dx, at, rows, V, A, stream);
+}
+
+template <typename T, int NT, int NV, bool KEEP>
 bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    const bool two = A.alpha < 1.0f && A.targets && A.temperature != 1.0f;
-    if (A.rest) return two ? dis_run<T, NT, NV, true, true>(x, dx, at, rows, V, A, stream)
-                           : dis_run<T, NT, NV, true, false>(x, dx, at, rows, V, A, stream);
-    return two ? dis_run<T, NT, NV, false, true>(x, dx, at, rows, V, A, stream)
-               : dis_run<T, NT, NV, false, false>(x, dx, at, rows, V, A, stream);
+    return A.rest ? dis_hard<T, NT, NV, KEEP, true>(x, dx, at, rows, V, A, stream)
+                  : dis_hard<T, NT, NV, KEEP, false>(x, dx, at, rows, V, A, stream);
 }
 
 // the smallest workgroup whose registers hold a row
 template <typename T>
 bool dis_launch(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
     const int vectors = (V + 2 * SaVec<T>::N - 2) / SaVec<T>::N;
-    if (vectors <= 64 * 2) return dis_pick<T, 64, 2>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 256 * 8) return dis_pick<T, 256, 8>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 512 * 16) return dis_pick<T, 512, 16>(x, dx, at, rows, V, A, stream);
-    return dis_pick<T, 1024, 16>(x, dx, at, rows, V, A, stream);
+    constexpr int VEC = SaVec<T>::N;  // (a thread keeps at most 64 exponentials)
+    if (vectors <= 64 * 2) return dis_pick<T, 64, 2, true>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 256 * 4) return dis_pick<T, 256, 4, true>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 512 * 32 / VEC) return dis_pick<T, 512, 32 / VEC, true>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 512 * 64 / VEC) return dis_pick<T, 512, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
+    return dis_pick<T, 1024, 16, VEC == 4>(x, dx, at, rows, V, A, stream);
 }
 
 }  // namespace
