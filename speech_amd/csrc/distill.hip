@@ -36,12 +36,14 @@ __device__ __forceinline__ float dis_base(float m) { return m == -INFINITY ? 0.0
 
 // REST: the rest is a class, and the list is taken out of the sums.  The sum at temperature 1 beside the one at T, HARD: 0 not wanted
 // or the same; 1 by its own exponential; 2, 4 as that power of the one at T = 2, 4.
-template <typename T, int NT, int NV, bool KEEP, bool REST, int HARD>
-__global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, DisArgs A) {
+// MORE: rows longer than the registers hold.
+template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST, int HARD>
+__global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, int stash, DisArgs A) {
     constexpr int VEC = SaVec<T>::N, NW = NT / 64;
     constexpr bool TWO = HARD != 0;
     static_assert(!KEEP || HARD != 1, "only one exponential of an element is kept");
-    extern __shared__ unsigned bitmap[];  // a bit per element of the row's vectors: the token is in the list
+    extern __shared__ uint4 held[];                // `stash` vectors a thread, and behind them
+    unsigned* bitmap = (unsigned*)(held + stash * NT);  // a bit per element of the row's vectors: the token is in the list
     __shared__ DisSum waves[NW];
     __shared__ int ids[SA_TOP_MAX];
     __shared__ float qs[SA_TOP_MAX];
@@ -73,6 +75,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, (i * NT + tid) * VEC - lead, V);
+    const long long target = A.alpha < 1.0f && A.targets ? A.targets[row] : -1;
+    const bool hard = target >= 0 && target < V;
+    const float xt = hard ? sa_widen(xr[target]) : 0.0f;
     // the list: marked in the bitmap by the first wave, two entries a lane
     int id[2] = {-1, -1};
     float a[2] = {-INFINITY, -INFINITY}, xv[2] = {-INFINITY, -INFINITY};
@@ -109,11 +114,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
     float q[2], qsum[2], am = 0.0f, lt = 0.0f, qr = 0.0f, ar = -INFINITY;
     if (tid < 64) {
         if (REST) ar = A.rest[row];
-        am = fmaxf(sa_wave_max(fmaxf(a[0], a[1])), ar);
+        am = fmaxf(sa_wave_max_dpp(fmaxf(a[0], a[1])), ar);
         soft = am > -INFINITY && A.alpha > 0.0f;
         const float e0 = soft ? sa_exp2((a[0] - am) * SA_LOG2E) : 0.0f, e1 = soft ? sa_exp2((a[1] - am) * SA_LOG2E) : 0.0f;
         const float er = soft && REST ? sa_exp2((ar - am) * SA_LOG2E) : 0.0f;
-        const float total = sa_wave_sum(e0 + e1) + er;
+        const float total = sa_wave_sum_dpp(e0 + e1) + er;
         lt = logf(total);
         q[0] = soft ? e0 / total : 0.0f;
         q[1] = soft ? e1 / total : 0.0f;
@@ -140,9 +145,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
         }
         if (REST) {
             const float y0 = first[0] ? xv[0] : -INFINITY, y1 = first[1] ? xv[1] : -INFINITY;
-            const float mt = sa_wave_max(fmaxf(y0, y1)), b = dis_base(mt);
-            const float st = sa_wave_sum(sa_exp2((y0 - b) * c) + sa_exp2((y1 - b) * c));
-            const float ht = TWO ? sa_wave_sum(sa_exp2((y0 - b) * SA_LOG2E) + sa_exp2((y1 - b) * SA_LOG2E)) : st;
+            const float mt = sa_wave_max_dpp(fmaxf(y0, y1)), b = dis_base(mt);
+            const float st = sa_wave_sum_dpp(sa_exp2((y0 - b) * c) + sa_exp2((y1 - b) * c));
+            const float ht = TWO ? sa_wave_sum_dpp(sa_exp2((y0 - b) * SA_LOG2E) + sa_exp2((y1 - b) * SA_LOG2E)) : st;
             if (lane == 0) { list[0] = mt; list[1] = st; list[2] = ht; }
         }
         if (lane == 0) { list[3] = qr; soft_row = soft; }
@@ -189,22 +194,31 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
             again(raw[i]);
         }
     }
-    for (int p = NV * NT + tid; p < nq; p += NT) {  // what the registers did not hold
-        uint4 r = sa_load_vec(xr, p * VEC - lead, V);
-        if (REST) drop(r, p);
+    // what the registers do not hold: the next `stash` vectors of a thread stay in LDS, the others are read again
+    for (int i = NV; MORE && i * NT < nq; i += 4) {
+        uint4 r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r[u] = sa_load_vec(xr, ((i + u) * NT + tid) * VEC - lead, V);
         float m = d.m;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) m = fmaxf(m, sa_element<T>(r, e));
+        for (int u = 0; u < 4; ++u) {
+            if (REST && (i + u) * NT + tid < nq) drop(r[u], (i + u) * NT + tid);
+            if (i + u - NV < stash) held[(i + u - NV) * NT + tid] = r[u];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = fmaxf(m, sa_element<T>(r[u], e));
+        }
         const float b = dis_base(m), o = d.m - b;
         d.s *= sa_exp2(o * c);
         if (TWO) d.h *= sa_exp2(o * SA_LOG2E);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float t = sa_element<T>(r, e) - b, u = sa_exp2(t * c);
-            d.s += u;
-            if (HARD == 1) d.h += sa_exp2(t * SA_LOG2E);
-            if (HARD > 1) d.h += power(u);
-        }
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float t = sa_element<T>(r[u], e) - b, g = sa_exp2(t * c);
+                d.s += g;
+                if (HARD == 1) d.h += sa_exp2(t * SA_LOG2E);
+                if (HARD > 1) d.h += power(g);
+            }
         d.m = m;
     }
     {   // the wave, then the waves in their order
@@ -239,8 +253,6 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
         qr = list[3];
     }
     soft = soft_row != 0;
-    const long long target = A.alpha < 1.0f && A.targets ? A.targets[row] : -1;
-    const bool hard = target >= 0 && target < V;
 
     if (A.loss_rows && tid < 64) {
         const float lS = logf(S);
@@ -248,11 +260,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (q[i] > 0.0f) l += q[i] * ((a[i] - am) - lt - ((xv[i] - m) / A.temperature - lS));
-        l = sa_wave_sum(l);
+        l = sa_wave_sum_dpp(l);
         if (lane == 0) {
             if (REST && qr > 0.0f) l += qr * ((ar - am) - lt - ((mr - m) / A.temperature + logf(sr) - lS));
             float v = soft ? A.alpha * A.temperature * A.temperature * l : 0.0f;
-            if (hard) v += (1.0f - A.alpha) * (logf(H) - (sa_widen(xr[target]) - m));
+            if (hard) v += (1.0f - A.alpha) * (logf(H) - (xt - m));
             A.loss_rows[row] = f * v;
         }
     }
@@ -297,9 +309,14 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
             grad(raw[i], p);
         }
     }
-    for (int p = NV * NT + tid; p < nq; p += NT) {
-        uint4 r = sa_load_vec(xr, p * VEC - lead, V);
-        grad(r, p);
+    for (int i = NV; MORE && i * NT < nq; i += 4) {
+        uint4 r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            r[u] = i + u - NV < stash ? held[(i + u - NV) * NT + tid] : sa_load_vec(xr, ((i + u) * NT + tid) * VEC - lead, V);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if ((i + u) * NT + tid < nq) grad(r[u], (i + u) * NT + tid);
     }
     __syncthreads();
     if (tid < 64) {
@@ -311,7 +328,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
                 dr[id[i]] = sa_narrow<T>(g);
             }
         if (lane == 0 && hard && !((bitmap[(target + lead) >> 5] >> ((target + lead) & 31)) & 1u)) {
-            const float t = sa_widen(xr[target]) - br;
+            const float t = xt - br;
             const float g = (TWO ? kr * sa_exp2(t * c) + kh * sa_exp2(t * SA_LOG2E) : kr * sa_exp2(t * c)) - ch;
             dr[target] = sa_narrow<T>(g);
         }
@@ -333,41 +350,51 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     }
 }
 
-template <typename T, int NT, int NV, bool KEEP, bool REST, int HARD>
+template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST, int HARD>
 bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    const size_t smem = (size_t)((V + 2 * SaVec<T>::N + 31) / 32) * 4;
-    constexpr auto kernel = distill_kernel<T, NT, NV, KEEP && HARD != 1, REST, HARD>;
+    // rows beyond the registers: as many vectors as 152 KB of LDS hold beside the bitmap
+    const size_t bits = (size_t)((V + 2 * SaVec<T>::N + 31) / 32) * 4;
+    const int more = (V + 2 * SaVec<T>::N - 2) / SaVec<T>::N - NT * NV;
+    int stash = MORE && more > 0 ? (int)((152 * 1024 - bits) / (16 * NT)) : 0;
+    if (stash * NT > more) stash = more > 0 ? (more + NT - 1) / NT : 0;
+    const size_t smem = bits + (size_t)stash * NT * 16;
+    constexpr auto kernel = distill_kernel<T, NT, NV, KEEP && HARD != 1, MORE, REST, HARD>;
     if (smem > 48 * 1024 &&
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
         return false;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(NT), smem, stream, (const T*)x, (T*)dx, at, V, A);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(NT), smem, stream, (const T*)x, (T*)dx, at, V, stash, A);
     return true;
 }
 
-template <typename T, int NT, int NV, bool KEEP, bool REST>
+template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST>
 bool dis_hard(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    if (A.alpha == 1.0f || !A.targets || A.temperature == 1.0f) return dis_run<T, NT, NV, KEEP, REST, 0>(x, dx, at, rows, V, A, stream);
-    if (A.temperature == 2.0f) return dis_run<T, NT, NV, KEEP, REST, 2>(x, dx, at, rows, V, A, stream);
-    if (A.temperature == 4.0f) return dis_run<T, NT, NV, KEEP, REST, 4>(x, dx, at, rows, V, A, stream);
-    return dis_run<T, NT, NV, KEEP, REST, 1>(x, dx, at, rows, V, A, stream);
+    if (A.alpha == 1.0f || !A.targets || A.temperature == 1.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 0>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 2.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 2>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 4.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 4>(x, dx, at, rows, V, A, stream);
+    return dis_run<T, NT, NV, KEEP, MORE, REST, 1>(x, dx, at, rows, V, A, stream);
 }
 
-template <typename T, int NT, int NV, bool KEEP>
+template <typename T, int NT, int NV, bool KEEP, bool MORE = false>
 bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    return A.rest ? dis_hard<T, NT, NV, KEEP, true>(x, dx, at, rows, V, A, stream)
-                  : dis_hard<T, NT, NV, KEEP, false>(x, dx, at, rows, V, A, stream);
+    return A.rest ? dis_hard<T, NT, NV, KEEP, MORE, true>(x, dx, at, rows, V, A, stream)
+                  : dis_hard<T, NT, NV, KEEP, MORE, false>(x, dx, at, rows, V, A, stream);
 }
 
-// the smallest workgroup whose registers hold a row
+// The smallest workgroup whose registers hold a row, 64 exponentials a thread at most: up to 128 registers a thread, so that the
+// 512-thread ones run two to a CU and one stores while the other loads (4096 x 32000 bf16: 110 us with 512 threads, 134 with 256,
+// 185 with 1024; recomputing the exponentials from 16-bit logits takes a third of the registers and 124 us).  A row beyond that
+// keeps what it can in LDS: 1024 threads, 256 KB in registers and 128 KB in LDS (2048 x 131072 f32: 440 us; without LDS 534, two
+// smaller workgroups on a CU 580 - 615, all of them bound by what is read twice).
 template <typename T>
 bool dis_launch(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    const int vectors = (V + 2 * SaVec<T>::N - 2) / SaVec<T>::N;
-    constexpr int VEC = SaVec<T>::N;  // (a thread keeps at most 64 exponentials)
+    constexpr int VEC = SaVec<T>::N;
+    const int vectors = (V + 2 * VEC - 2) / VEC;
     if (vectors <= 64 * 2) return dis_pick<T, 64, 2, true>(x, dx, at, rows, V, A, stream);
     if (vectors <= 256 * 4) return dis_pick<T, 256, 4, true>(x, dx, at, rows, V, A, stream);
     if (vectors <= 512 * 32 / VEC) return dis_pick<T, 512, 32 / VEC, true>(x, dx, at, rows, V, A, stream);
     if (vectors <= 512 * 64 / VEC) return dis_pick<T, 512, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
-    return dis_pick<T, 1024, 16, VEC == 4>(x, dx, at, rows, V, A, stream);
+    if (vectors <= 1024 * 64 / VEC) return dis_pick<T, 1024, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
+    return dis_pick<T, 1024, 64 / VEC, true, true>(x, dx, at, rows, V, A, stream);
 }
 
 }  // namespace

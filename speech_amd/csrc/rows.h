@@ -125,7 +125,11 @@ template <> __device__ __forceinline__ uint4 sa_pack<SaF16>(const float* g) {
 // the vector whose first element is v0, into a row that starts at the same offset from a 16-byte boundary
 template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v0, int V, const float* g, bool aligned) {
     if (aligned && v0 >= 0 && v0 + SaVec<T>::N <= V) {
-        *reinterpret_cast<uint4*>(row + v0) = sa_pack<T>(g);
+        // (past the caches: what is written here is as large as what is read, and reads again come first; 2048 x 131072 f32 gradients
+        // 470 -> 440 us)
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        const uint4 w = sa_pack<T>(g);
+        __builtin_nontemporal_store((u4){w.x, w.y, w.z, w.w}, reinterpret_cast<u4*>(row + v0));
         return;
     }
 #pragma unroll
