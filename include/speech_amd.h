@@ -598,7 +598,7 @@ typedef struct {
 
 ctcStatus_t sa_logits_constrain(const void* x, long ldx, int dtype, void* y, long ldy, int rows, int V,
                                 const saConstraints* c, void* stream);
-size_t sa_logits_pick_workspace_bytes(int rows, int V);
+size_t sa_logits_pick_workspace_bytes(int rows, int V, int dtype);
 ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int rows, int V, const saConstraints* c,
                            long long* d_tokens, float* d_logp, void* workspace, size_t workspace_bytes, void* stream);
 

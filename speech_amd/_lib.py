@@ -152,7 +152,7 @@ SIGNATURES = {
     "sa_argmax_rows": (c_int, [c_void_p, c_void_p, c_long, c_int, c_void_p]),
     "sa_logits_constrain": (c_int, [c_void_p, c_long, c_int, c_void_p, c_long, c_int, c_int,
                                     ctypes.POINTER(saConstraints), c_void_p]),
-    "sa_logits_pick_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "sa_logits_pick_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "sa_logits_pick": (c_int, [c_void_p, c_long, c_int, c_int, c_int, ctypes.POINTER(saConstraints), c_void_p, c_void_p,
                                c_void_p, c_size_t, c_void_p]),
     "sa_top_logits_workspace_bytes": (c_size_t, [c_long, c_int, c_int, c_int]),

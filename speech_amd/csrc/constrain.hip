@@ -1,15 +1,15 @@
 // constrain.hip -- penalties for repeated tokens, biases and grammar masks on output rows, and the token that is left
 // (sa_logits_constrain, sa_logits_pick; the arithmetic is stated in include/speech_amd.h).
 //
-// A workgroup takes a segment of a row.  What the history and the bias list say about the segment's tokens is gathered in LDS
-// first, one 32-bit word a token: the low half counts the token in the history, the high half holds 1 + the position of the
-// last bias entry of that token (hence the limit of 65535 on both lists).  Integer maxima and sums: the order in which the
-// lanes arrive does not matter.  The row itself is read once.
+// A workgroup takes a segment of a row and reads it once, as 16-byte vectors, into registers.  Meanwhile the history and the bias
+// list are gathered in LDS, one 32-bit word a token of the segment: the low half counts the token in the history, the high half
+// holds 1 + the position of the last bias entry of that token (hence the limit of 65535 on both lists).  Integer maxima and
+// sums: the order in which the lanes arrive does not matter.  The few tokens that are found there are collected, and their final
+// logits -- the division and the other steps that most tokens do not need -- take the place of their words.  Then every element is
+// either its logit or its word, masked, and stored or reduced.
 #include "rows.h"
 
 namespace {
-
-constexpr int kConThreads = 256, kConEach = 16, kConSeg = kConThreads * kConEach;
 
 struct PickPart {  // what a segment leaves for its row: the best token, the maximum and the sum of exp(x - maximum)
     unsigned long long key;
@@ -19,10 +19,8 @@ struct PickPart {  // what a segment leaves for its row: the best token, the max
 // exp(x - m) where equal infinities count as equal (a bias of +inf forces its token)
 __device__ __forceinline__ float con_exp(float x, float m) { return x == m ? 1.0f : sa_exp2((x - m) * SA_LOG2E); }
 
-template <typename T>
-__device__ __forceinline__ float con_value(T raw, unsigned word, bool allowed, float r, float p, float f, const float* bias) {
+__device__ __forceinline__ float con_value(float x, unsigned word, float r, float p, float f, const float* bias) {
 #pragma clang fp contract(off)  // every step is rounded as the formula is written: the token must not depend on a fused step
-    float x = sa_widen(raw);
     const unsigned c = word & 0xffffu, b = word >> 16;
     if (c) {
         x = x > 0.0f ? x / r : x * r;
@@ -30,94 +28,148 @@ __device__ __forceinline__ float con_value(T raw, unsigned word, bool allowed, f
         x = x - p;
     }
     if (b) x = x + bias[b - 1];
-    return allowed ? x : -INFINITY;
+    return x;
 }
 
-// The two lists of `row`, for the tokens [v0, v0 + n): every thread of the block calls it.
-__device__ __forceinline__ void con_lists(unsigned* words, const saConstraints& C, int row, int v0, int n) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) words[i] = 0;
-    __syncthreads();
-    if (C.bias_ids) {
-        const long long* ids = C.bias_ids + (long)row * C.bias_ld;
-        for (int j = threadIdx.x; j < C.n_bias; j += blockDim.x) {
-            const unsigned long long d = (unsigned long long)(ids[j] - v0);
-            if (d < (unsigned long long)n) atomicMax(&words[d], (unsigned)(j + 1) << 16);
-        }
-        __syncthreads();
-    }
-    if (C.history) {
-        const long long* h = C.history + (long)row * C.history_ld;
-        int len = C.lengths ? C.lengths[row] : C.history_len;
-        len = len < 0 ? 0 : (len > C.history_len ? C.history_len : len);
-        for (int i = threadIdx.x; i < len; i += blockDim.x) {
-            const unsigned long long d = (unsigned long long)(h[i] - v0);
-            if (d < (unsigned long long)n) atomicAdd(&words[d], 1u);
-        }
-    }
-    __syncthreads();
+// bits v0 .. v0 + VEC - 1 of a mask row (bits of tokens outside [0, V) are not looked at by anybody)
+template <int VEC> __device__ __forceinline__ unsigned con_allowed(const unsigned* __restrict__ mask, int v0, int V) {
+    const int lo = v0 < 0 ? 0 : v0 >> 5, last = (V - 1) >> 5, hi = (v0 + VEC - 1) >> 5;
+    const unsigned a = mask[lo > last ? last : lo], b = mask[hi < 0 ? 0 : hi > last ? last : hi];
+    if (v0 < 0) return a << -v0;
+    return (unsigned)(((((unsigned long long)b) << 32 | a)) >> (v0 & 31));
 }
 
-template <typename T, bool PICK>
-__global__ __launch_bounds__(kConThreads) void constrain_kernel(const T* __restrict__ x, long ldx, T* y, long ldy, int V,
-                                                                int nseg, saConstraints C, PickPart* __restrict__ part,
-                                                                long long* __restrict__ tokens, float* __restrict__ logp) {
-    __shared__ unsigned words[kConSeg];
-    __shared__ float scratch[kConThreads / 64];
-    __shared__ unsigned long long best[kConThreads / 64];
+template <typename T, int NV, bool PICK>
+__global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T* y /* may be x */, long ldy, int V, int nseg, int per,
+                                                        saConstraints C, PickPart* __restrict__ part, long long* __restrict__ tokens,
+                                                        float* __restrict__ logp) {
+    constexpr int VEC = SaVec<T>::N, NT = 256, SEG = NT * NV * VEC;
+    extern __shared__ unsigned words[];  // SEG words, then SEG positions (16 bits); nothing where there are no lists
+    __shared__ int found;
+    __shared__ float scratch[NT / 64];
+    __shared__ unsigned long long best[NT / 64];
     const int row = blockIdx.x / nseg, seg = blockIdx.x % nseg, tid = threadIdx.x;
-    const int v0 = seg * kConSeg, n = V - v0 < kConSeg ? V - v0 : kConSeg;
-    con_lists(words, C, row, v0, n);
-    const float r = C.repetition ? C.repetition[row] : C.repetition_all;
-    const float p = C.presence ? C.presence[row] : C.presence_all;
-    const float f = C.frequency ? C.frequency[row] : C.frequency_all;
-    const float* bias = C.bias_values + (long)row * C.bias_ld;
+    const T* xr = x + (long)row * ldx;
+    const int first = seg * per * VEC - sa_lead(xr), end = first + per * VEC < V ? first + per * VEC : V;
+    uint4 raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, first + (i * NT + tid) * VEC, end);
     const unsigned* mask = nullptr;
     if (C.mask) {
         const int state = C.states ? C.states[row] : row;
         if (state >= 0 && state < C.n_states) mask = C.mask + (long)state * C.mask_ld;
     }
-    const T* xr = x + (long)row * ldx + v0;
-    float val[kConEach];
-    unsigned long long key = 0;
-    float m = -INFINITY;
+    const bool lists = C.history || C.bias_ids;
+    if (lists) {
+        sa_u16* places = (sa_u16*)(words + SEG);
+        const float r = C.repetition ? C.repetition[row] : C.repetition_all;
+        const float p = C.presence ? C.presence[row] : C.presence_all;
+        const float f = C.frequency ? C.frequency[row] : C.frequency_all;
+        const float* bias = C.bias_values + (long)row * C.bias_ld;
+        int len = 0;
+        if (C.history) {
+            len = C.lengths ? C.lengths[row] : C.history_len;
+            len = len < 0 ? 0 : (len > C.history_len ? C.history_len : len);
+        }
+        uint4* clear = (uint4*)words;
 #pragma unroll
-    for (int j = 0; j < kConEach; ++j) {
-        const int i = tid + j * kConThreads;
-        val[j] = -INFINITY;
-        if (i < n) {
-            const int v = v0 + i;
-            const bool allowed = !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
-            val[j] = con_value(xr[i], words[i], allowed, r, p, f, bias);
-            if (PICK) {
-                const unsigned long long k = sa_rank_key(val[j], v);
-                key = k > key ? k : key;
-                m = fmaxf(m, val[j]);
-            } else {
-                y[(long)row * ldy + v] = sa_narrow<T>(val[j]);
+        for (int i = 0; i < SEG / 4 / NT; ++i) clear[i * NT + tid] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) found = 0;
+        // (a token t of a list is the segment's when `first` <= t < `end`; t >= 0 keeps what lies before the row out; the last
+        // segment of a row that starts on a boundary may be empty, and begin behind the row's end)
+        const unsigned long long n = end > first ? (unsigned long long)(end - first) : 0ull;
+        __syncthreads();
+        if (C.bias_ids) {
+            const long long* ids = C.bias_ids + (long)row * C.bias_ld;
+            for (int j = tid; j < C.n_bias; j += NT) {
+                const long long t = ids[j];
+                const unsigned long long d = (unsigned long long)(t - first);
+                if (t >= 0 && d < n && atomicMax(&words[d], (unsigned)(j + 1) << 16) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
+            }
+            __syncthreads();
+        }
+        if (len > 0) {
+            const long long* h = C.history + (long)row * C.history_ld;
+#pragma unroll 4
+            for (int i = tid; i < len; i += NT) {
+                const long long t = h[i];
+                const unsigned long long d = (unsigned long long)(t - first);
+                if (t >= 0 && d < n && atomicAdd(&words[d], 1u) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
             }
         }
+        __syncthreads();
+        for (int i = tid; i < found; i += NT) {
+            const int d = places[i];
+            const unsigned u = __builtin_bit_cast(unsigned, con_value(sa_widen(xr[first + d]), words[d], r, p, f, bias));
+            words[d] = u ? u : 0x80000000u;  // (0 marks a token that is in no list)
+        }
+        __syncthreads();
     }
-    if (!PICK) return;
+    T* yr = PICK ? nullptr : y + (long)row * ldy;
+    const bool aligned = !PICK && sa_lead(yr) == sa_lead(xr);
+    unsigned long long key = 0;
+    float m = -INFINITY, val[PICK ? NV * VEC : VEC];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor(key, o, 64);
-        key = other > key ? other : key;
-    }
-    if ((tid & 63) == 0) best[tid >> 6] = key;
-    m = sa_block_max<kConThreads / 64>(m, scratch);  // (its barriers also publish `best`)
-    float s = 0.f;
+    for (int i = 0; i < NV; ++i) {
+        const int q = i * NT + tid, v0 = first + q * VEC;
+        if (v0 >= end) {
+            if (PICK)
 #pragma unroll
-    for (int j = 0; j < kConEach; ++j)
-        if (tid + j * kConThreads < n) s += con_exp(val[j], m);
-    s = sa_block_sum<kConThreads / 64>(s, scratch);
-    if (tid == 0) {
-        for (int w = 0; w < kConThreads / 64; ++w) key = best[w] > key ? best[w] : key;
-        if (nseg == 1) {
-            const bool none = (unsigned)(key >> 32) == sa_order(-INFINITY);
-            tokens[row] = none ? -1 : (long long)(unsigned)~(unsigned)key;
-            logp[row] = none ? -INFINITY : -logf(s);
+                for (int e = 0; e < VEC; ++e) val[i * VEC + e] = -INFINITY;
+            continue;
+        }
+        float* g = val + (PICK ? i * VEC : 0);
+        const unsigned allowed = mask ? con_allowed<VEC>(mask, v0, V) : ~0u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            g[e] = sa_element<T>(raw[i], e);
+            if (lists) {
+                const unsigned w = words[q * VEC + e];
+                g[e] = w ? __builtin_bit_cast(float, w) : g[e];
+            }
+            g[e] = (allowed >> e) & 1u ? g[e] : -INFINITY;
+        }
+        if constexpr (PICK) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (v0 + e >= 0 && v0 + e < end) {
+                    const unsigned long long k = sa_rank_key(g[e], v0 + e);
+                    key = k > key ? k : key;
+                    m = fmaxf(m, g[e]);
+                } else {
+                    g[e] = -INFINITY;
+                }
+            }
         } else {
-            part[blockIdx.x] = PickPart{key, m, s};
+            sa_store_vec<T>(yr, v0, end, g, aligned);
+        }
+    }
+    if constexpr (PICK) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const unsigned long long other = __shfl_xor(key, o, 64);
+            key = other > key ? other : key;
+        }
+        if ((tid & 63) == 0) best[tid >> 6] = key;
+        m = sa_block_max<NT / 64>(m, scratch);  // (its barriers also publish `best`)
+        float s = 0.0f;
+        if (m > -INFINITY) {  // (else every exponential would be that of equal infinities; nothing is left anyway)
+#pragma unroll
+            for (int i = 0; i < NV * VEC; ++i) s += con_exp(val[i], m);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV * VEC; ++i) s += val[i] == val[i] ? 0.0f : NAN;
+        }
+        s = sa_block_sum<NT / 64>(s, scratch);
+        if (tid == 0) {
+            for (int w = 0; w < NT / 64; ++w) key = best[w] > key ? best[w] : key;
+            if (nseg == 1) {
+                const bool none = (unsigned)(key >> 32) == sa_order(-INFINITY);
+                tokens[row] = none ? -1 : (long long)(unsigned)~(unsigned)key;
+                logp[row] = none ? -INFINITY : -logf(s);
+            } else {
+                part[blockIdx.x] = PickPart{key, m, s};
+            }
         }
     }
 }
@@ -139,7 +191,8 @@ __global__ __launch_bounds__(64) void pick_join_kernel(const PickPart* __restric
     }
     m = sa_wave_max(m);
     float s = 0.f;
-    for (int i = threadIdx.x; i < nseg; i += 64) s += P[i].s * con_exp(P[i].m, m);
+    for (int i = threadIdx.x; i < nseg; i += 64)
+        if (P[i].m > -INFINITY || P[i].s != 0.0f) s += P[i].s * con_exp(P[i].m, m);
     s = sa_wave_sum(s);
     if (threadIdx.x == 0) {
         const bool none = (unsigned)(key >> 32) == sa_order(-INFINITY);
@@ -148,7 +201,21 @@ __global__ __launch_bounds__(64) void pick_join_kernel(const PickPart* __restric
     }
 }
 
-int con_segments(int V) { return (V + kConSeg - 1) / kConSeg; }
+// Vectors a thread, segments a row, vectors a segment.  Segments as long as the registers and 48 KB of LDS allow -- each reads
+// the lists of its row again -- unless that leaves CUs without work; a row that one workgroup can hold is not split where that
+// would cost pick a second launch.
+struct ConPlan { int nv, nseg, per; };
+ConPlan con_plan(int rows, int V, int dtype, bool pick) {
+    const int vec = dtype == SA_F32 ? 4 : 8, most = dtype == SA_F32 ? 8 : 4, vectors = (V + 2 * vec - 2) / vec;
+    ConPlan p{1, 1, 0};
+    while (p.nv < most && 256 * p.nv < vectors &&
+           ((pick && vectors <= 256 * most) || (long)rows * ((vectors + 512 * p.nv - 1) / (512 * p.nv)) >= 512))
+        p.nv *= 2;
+    p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
+    p.per = (vectors + p.nseg - 1) / p.nseg;
+    p.nseg = (vectors + p.per - 1) / p.per;
+    return p;
+}
 
 bool con_ok(const saConstraints* c, int rows, int V) {
     if (!c || c->history_len < 0 || c->history_len > SA_LIST_MAX || c->n_bias < 0 || c->n_bias > SA_LIST_MAX) return false;
@@ -166,21 +233,28 @@ saConstraints con_used(const saConstraints& c) {
     return u;
 }
 
-template <bool PICK>
-void con_launch(const void* x, long ldx, int dtype, void* y, long ldy, int rows, int V, const saConstraints& c, PickPart* part,
-                long long* tokens, float* logp, hipStream_t stream) {
+template <typename T, bool PICK>
+void con_launch(const void* x, long ldx, void* y, long ldy, int rows, int V, const ConPlan& p, const saConstraints& c,
+                PickPart* part, long long* tokens, float* logp, hipStream_t stream) {
     const saConstraints C = con_used(c);
-    const int nseg = con_segments(V);
-    const dim3 grid((unsigned)((size_t)rows * nseg)), block(kConThreads);
-    if (dtype == SA_F32)
-        hipLaunchKernelGGL((constrain_kernel<float, PICK>), grid, block, 0, stream, (const float*)x, ldx, (float*)y, ldy, V, nseg, C,
-                           part, tokens, logp);
-    else if (dtype == SA_BF16)
-        hipLaunchKernelGGL((constrain_kernel<SaBf16, PICK>), grid, block, 0, stream, (const SaBf16*)x, ldx, (SaBf16*)y, ldy, V,
-                           nseg, C, part, tokens, logp);
-    else
-        hipLaunchKernelGGL((constrain_kernel<SaF16, PICK>), grid, block, 0, stream, (const SaF16*)x, ldx, (SaF16*)y, ldy, V, nseg,
-                           C, part, tokens, logp);
+    const dim3 grid((unsigned)((size_t)rows * p.nseg)), block(256);
+    const size_t smem = C.history || C.bias_ids ? (size_t)256 * p.nv * SaVec<T>::N * 6 : 0;
+#define CON_LAUNCH(NV)                                                                                                        \
+    hipLaunchKernelGGL((constrain_kernel<T, NV, PICK>), grid, block, smem, stream, (const T*)x, ldx, (T*)y, ldy, V, p.nseg, p.per, \
+                       C, part, tokens, logp)
+    if (p.nv == 1) CON_LAUNCH(1);
+    else if (p.nv == 2) CON_LAUNCH(2);
+    else if (p.nv == 4) CON_LAUNCH(4);
+    else if constexpr (sizeof(T) == 4) CON_LAUNCH(8);
+#undef CON_LAUNCH
+}
+
+template <bool PICK>
+void con_run(const void* x, long ldx, int dtype, void* y, long ldy, int rows, int V, const ConPlan& p, const saConstraints& c,
+             PickPart* part, long long* tokens, float* logp, hipStream_t stream) {
+    if (dtype == SA_F32) con_launch<float, PICK>(x, ldx, y, ldy, rows, V, p, c, part, tokens, logp, stream);
+    else if (dtype == SA_BF16) con_launch<SaBf16, PICK>(x, ldx, y, ldy, rows, V, p, c, part, tokens, logp, stream);
+    else con_launch<SaF16, PICK>(x, ldx, y, ldy, rows, V, p, c, part, tokens, logp, stream);
 }
 
 }  // namespace
@@ -190,15 +264,17 @@ extern "C" ctcStatus_t sa_logits_constrain(const void* x, long ldx, int dtype, v
     SA_CLEAR_ERR();
     if (rows < 0 || !sa_rows_ok(dtype, V) || !con_ok(c, rows, V)) return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
-    if (!x || !y || (size_t)rows * con_segments(V) > 0x7fffffffu) return CTC_STATUS_INVALID_VALUE;
-    con_launch<false>(x, ldx, dtype, y, ldy, rows, V, *c, nullptr, nullptr, nullptr, (hipStream_t)stream);
+    const ConPlan p = con_plan(rows, V, dtype, false);
+    if (!x || !y || (size_t)rows * p.nseg > 0x7fffffffu) return CTC_STATUS_INVALID_VALUE;
+    con_run<false>(x, ldx, dtype, y, ldy, rows, V, p, *c, nullptr, nullptr, nullptr, (hipStream_t)stream);
     SA_CHECK_LAUNCH();
     return CTC_STATUS_SUCCESS;
 }
 
-extern "C" size_t sa_logits_pick_workspace_bytes(int rows, int V) {
-    if (rows < 1 || V < 1 || V > SA_VOCAB_MAX || con_segments(V) == 1) return 0;
-    return (size_t)rows * con_segments(V) * sizeof(PickPart);
+extern "C" size_t sa_logits_pick_workspace_bytes(int rows, int V, int dtype) {
+    if (rows < 1 || !sa_rows_ok(dtype, V)) return 0;
+    const ConPlan p = con_plan(rows, V, dtype, true);
+    return p.nseg == 1 ? 0 : (size_t)rows * p.nseg * sizeof(PickPart);
 }
 
 extern "C" ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int rows, int V, const saConstraints* c,
@@ -207,14 +283,14 @@ extern "C" ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int ro
     SA_CLEAR_ERR();
     if (rows < 0 || !sa_rows_ok(dtype, V) || !con_ok(c, rows, V)) return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
-    const size_t need = sa_logits_pick_workspace_bytes(rows, V);
-    if (!x || !d_tokens || !d_logp || (need && (!workspace || workspace_bytes < need)) ||
-        (size_t)rows * con_segments(V) > 0x7fffffffu)
+    const ConPlan p = con_plan(rows, V, dtype, true);
+    const size_t need = sa_logits_pick_workspace_bytes(rows, V, dtype);
+    if (!x || !d_tokens || !d_logp || (need && (!workspace || workspace_bytes < need)) || (size_t)rows * p.nseg > 0x7fffffffu)
         return CTC_STATUS_INVALID_VALUE;
-    con_launch<true>(x, ldx, dtype, nullptr, 0, rows, V, *c, (PickPart*)workspace, d_tokens, d_logp, (hipStream_t)stream);
+    con_run<true>(x, ldx, dtype, nullptr, 0, rows, V, p, *c, (PickPart*)workspace, d_tokens, d_logp, (hipStream_t)stream);
     if (need)
-        hipLaunchKernelGGL(pick_join_kernel, dim3(rows), dim3(64), 0, (hipStream_t)stream, (const PickPart*)workspace,
-                           con_segments(V), d_tokens, d_logp);
+        hipLaunchKernelGGL(pick_join_kernel, dim3(rows), dim3(64), 0, (hipStream_t)stream, (const PickPart*)workspace, p.nseg,
+                           d_tokens, d_logp);
     SA_CHECK_LAUNCH();
     return CTC_STATUS_SUCCESS;
 }

@@ -138,7 +138,7 @@ template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v
 }
 
 // the vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V)
-template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* __restrict__ row, int v0, int V) {
+template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* row, int v0, int V) {
     if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
     const unsigned f = sa_fill_word<T>();
     unsigned w[4] = {f, f, f, f};

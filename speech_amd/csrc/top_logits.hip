@@ -352,6 +352,7 @@ TopPlan top_plan(int V, int k, int dtype) {
     p.nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : vectors <= 1024 ? 4 : 8;
     p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
     p.per = (vectors + p.nseg - 1) / p.nseg;
+    p.nseg = (vectors + p.per - 1) / p.per;
     p.cap = k + k / 2 + 32;
     return p;
 }

@@ -66,21 +66,20 @@ def _tensor(t, name, dtype, shape, device):
     return t.data_ptr()
 
 
-class _on:
-    """The device of the logits as the current one, and its current stream."""
+_device_now = torch._C._cuda_getDevice                # (what torch.cuda.current_device() / current_stream() end up calling:
+_stream_now = torch._C._cuda_getCurrentRawStream      # a token's call is shorter than the objects those two build)
 
-    def __init__(self, x):
-        self.guard = None if torch.cuda.current_device() == x.device.index else torch.cuda.device(x.device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _launch(name, x, *args):
+    """Library entry `name` on the device of x and that device's current stream."""
+    fn, index = getattr(_lib.lib(), name), x.get_device()
+    if _device_now() == index:
+        status = fn(*args, _stream_now(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _stream_now(index))
+    if status != 0:
+        check(status, name)
 
 
 def pack_mask(allowed):
@@ -184,9 +183,8 @@ def constrain(logits, history=None, lengths=None, repetition=None, presence=None
             raise SpeechAmdError("out must be like the logits, without overlapping rows")
         if out.requires_grad and torch.is_grad_enabled():
             raise SpeechAmdError("constrain writes to out without recording it: out must not require a gradient")
-    with _on(logits) as stream:
-        check(_lib.lib().sa_logits_constrain(logits.data_ptr(), ld, _DTYPES[logits.dtype], out.data_ptr(),
-                                             out.stride(0), rows, V, ctypes.byref(c), stream), "sa_logits_constrain")
+    _launch("sa_logits_constrain", logits, logits.data_ptr(), ld, _DTYPES[logits.dtype], out.data_ptr(), out.stride(0), rows, V,
+            ctypes.byref(c))
     return out
 
 
@@ -200,13 +198,12 @@ def pick(logits, history=None, lengths=None, repetition=None, presence=None, fre
     c = _constraints(rows, V, dev, history, lengths, repetition, presence, frequency, bias_ids, bias_values, mask, states)
     tokens = torch.empty(rows, dtype=torch.int64, device=dev)
     logp = torch.empty(rows, dtype=torch.float32, device=dev)
-    L = _lib.lib()
-    with _on(logits) as stream:
-        nbytes = L.sa_logits_pick_workspace_bytes(rows, V)
-        # a workspace of the call's own: two streams, or two captured graphs, never share one
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(L.sa_logits_pick(logits.data_ptr(), ld, _DTYPES[logits.dtype], rows, V, ctypes.byref(c), tokens.data_ptr(),
-                               logp.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, stream), "sa_logits_pick")
+    code = _DTYPES[logits.dtype]
+    nbytes = _lib.lib().sa_logits_pick_workspace_bytes(rows, V, code)
+    # a workspace of the call's own: two streams, or two captured graphs, never share one
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch("sa_logits_pick", logits, logits.data_ptr(), ld, code, rows, V, ctypes.byref(c), tokens.data_ptr(), logp.data_ptr(),
+            ws.data_ptr() if nbytes else None, nbytes)
     return tokens, logp
 
 
@@ -229,14 +226,11 @@ def top_logits(logits, k, temperature=1.0):
     values = torch.empty(shape + (k,), dtype=torch.float32, device=dev)
     ids = torch.empty(shape + (k,), dtype=torch.int64, device=dev)
     rest = torch.empty(shape, dtype=torch.float32, device=dev)
-    L = _lib.lib()
     code = _DTYPES[logits.dtype]
-    with _on(logits) as stream:
-        nbytes = L.sa_top_logits_workspace_bytes(rows, V, k, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(L.sa_top_logits(logits.data_ptr(), ld_outer, ld_inner, n_inner, code, rows, V, k, t, values.data_ptr(),
-                              ids.data_ptr(), rest.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, stream),
-              "sa_top_logits")
+    nbytes = _lib.lib().sa_top_logits_workspace_bytes(rows, V, k, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch("sa_top_logits", logits, logits.data_ptr(), ld_outer, ld_inner, n_inner, code, rows, V, k, t, values.data_ptr(),
+            ids.data_ptr(), rest.data_ptr(), ws.data_ptr() if nbytes else None, nbytes)
     return values, ids, rest
 
 
@@ -262,10 +256,8 @@ class DistillFunction(torch.autograd.Function):
                 x = x.contiguous()
                 dx = torch.empty_like(x)
                 ld_outer, ld_inner, n_inner, rows = _rows_of(x)
-        with _on(x) as stream:
-            check(_lib.lib().sa_distill_loss(x.data_ptr(), None if dx is None else dx.data_ptr(), ld_outer, ld_inner, n_inner,
-                                             _DTYPES[x.dtype], rows, V, *args, None, 0, loss_rows.data_ptr(), loss.data_ptr(),
-                                             stream), "sa_distill_loss")
+        _launch("sa_distill_loss", x, x.data_ptr(), None if dx is None else dx.data_ptr(), ld_outer, ld_inner, n_inner,
+                _DTYPES[x.dtype], rows, V, *args, None, 0, loss_rows.data_ptr(), loss.data_ptr())
         if dx is not None:
             ctx.save_for_backward(x, values, ids, rest, targets, weights)
             ctx.args = (ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale)
@@ -288,10 +280,8 @@ class DistillFunction(torch.autograd.Function):
             dx = torch.empty_like(x)
         factor = go.detach().reshape(1).to(torch.float32)
         p = _lib.ptr
-        with _on(x) as stream:
-            check(_lib.lib().sa_distill_loss(p(x), p(dx), ld_outer, ld_inner, n_inner, _DTYPES[x.dtype], rows, V, p(values), p(ids),
-                                             p(rest), k, p(targets), p(weights), temperature, alpha, scale, p(factor),
-                                             0 if fresh else 1, None, None, stream), "sa_distill_loss")
+        _launch("sa_distill_loss", x, p(x), p(dx), ld_outer, ld_inner, n_inner, _DTYPES[x.dtype], rows, V, p(values), p(ids), p(rest), k,
+                p(targets), p(weights), temperature, alpha, scale, p(factor), 0 if fresh else 1, None, None)
         return (dx,) + none
 
 

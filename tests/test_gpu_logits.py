@@ -67,7 +67,8 @@ def constraints(g, n, V, length, biases, grammar, scalars=False):
 
 SHAPES = [(1, 1, 0, 0, True), (2, 29, 40, 3, True), (32, 29, 200, 0, True), (3, 32, 7, 50, False), (5, 1000, None, 9, True),
           (3, 4095, 300, 20, True), (2, 4096, 5000, 0, False), (4, 4097, 64, 64, True), (3, 8193, 600, 10, True), (2, 16385, 1, 1, True),
-          (2, 32000, 1500, 128, True), (7, 50021, 333, 16, True), (2, 131072, 4096, 100, True), (1, 262147, 70, 5, False)]
+          (2, 32000, 1500, 128, True), (7, 50021, 333, 16, True), (2, 131072, 4096, 100, True), (1, 262147, 70, 5, False),
+          (1, 1048576, 900, 300, True), (1, 1044481, 64, 0, False), (130, 8190, 20, 2, True)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -167,7 +168,11 @@ def test_constrain_in_place_on_rows_with_gaps(V, ld, off, dtype):
     other = torch.empty(n, ld + 3, dtype=dtype, device="cuda")[:, 3:3 + V]   # another alignment than the input's
     y = flat.cuda()[off:off + n * ld].view(n, ld)[:, :V]
     assert torch.equal(L().constrain(y, out=other, **cuda(kw)), want)
-    assert all(torch.equal(a, b) for a, b in zip(L().pick(y, **cuda(kw)), L().pick(y.contiguous(), **cuda(kw))))
+    (ta, la), (tb, lb) = L().pick(y, **cuda(kw)), L().pick(y.contiguous(), **cuda(kw))
+    assert torch.equal(ta, tb)
+    # the sum runs in another order where a row starts at another offset from a 16-byte boundary: each side is within the
+    # tolerance of a log-sum-exp (top of this file; |x - m| < 60 here) of the same number, so they are within twice that
+    assert float((la - lb).abs().max()) <= 2 * ((3 * 60 + 42) * U + 2 * U * float(la.abs().max()))
 
 
 def test_constrain_refuses_on_the_gpu():
@@ -202,7 +207,8 @@ def check_top(x, k, temperature=1.0, got=None):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("n,V,k", [(1, 1, 1), (5, 2, 2), (40, 29, 8), (700, 29, 29), (9, 64, 5), (9, 65, 33), (6, 128, 128), (3, 129, 128),
                                    (4, 511, 20), (4, 1000, 64), (3, 4099, 100), (2, 8192, 1), (2, 8195, 128), (3, 32000, 64),
-                                   (2, 50021, 100), (3, 131071, 128), (1, 300007, 50)])
+                                   (2, 50021, 100), (3, 131071, 128), (1, 300007, 50),
+                                   (1, 1048576, 128), (1, 1044483, 20)])
 def test_top_logits(n, V, k, dtype):
     check_top(rows_like(gen(V + k), n, V, dtype), k, 1.0 if n % 2 else 2.5)
 
@@ -362,7 +368,7 @@ def within(grad, loss, x, kw, temperature, alpha, denom=None, factor=None):
 
 
 DSHAPES = [(1, 1, 1), (3, 2, 1), (40, 29, 8), (7, 29, 29), (6, 64, 10), (5, 130, 100), (4, 513, 20), (3, 1000, 128), (5, 4099, 64), (6, 8193, 50),
-           (5, 32000, 64), (3, 50021, 20), (3, 70001, 64), (2, 131072, 128), (1, 300007, 30)]
+           (5, 32000, 64), (3, 50021, 20), (3, 70001, 64), (2, 131072, 128), (1, 300007, 30), (1, 1048576, 9)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
