@@ -140,18 +140,21 @@ template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v
 // the vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V)
 template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* row, int v0, int V) {
     if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
-    const unsigned f = sa_fill_word<T>();
-    unsigned w[4] = {f, f, f, f};
-#pragma unroll
+    // (a loop and not eight copies of its body: a row has two such vectors, and the registers of the others are wanted)
+    constexpr int BITS = 8 * (int)sizeof(T);
+    const unsigned long long f = (unsigned long long)sa_fill_word<T>() << 32 | sa_fill_word<T>();
+    unsigned long long w[2] = {f, f};
+#pragma unroll 1
     for (int e = 0; e < SaVec<T>::N; ++e) {
         const int v = v0 + e;
         if (v < 0 || v >= V) continue;
-        if constexpr (sizeof(T) == 4) {
-            w[e] = __builtin_bit_cast(unsigned, row[v]);
-        } else {
-            const unsigned h = __builtin_bit_cast(sa_u16, row[v]);
-            w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | (h << 16) : (w[e >> 1] & 0xffff0000u) | h;
-        }
+        unsigned long long h;
+        if constexpr (sizeof(T) == 4) h = __builtin_bit_cast(unsigned, row[v]);
+        else h = __builtin_bit_cast(sa_u16, row[v]);
+        const int at = e * BITS & 63;
+        const unsigned long long keep = ~(((1ull << BITS) - 1) << at);
+        if (e * BITS < 64) w[0] = (w[0] & keep) | h << at;
+        else w[1] = (w[1] & keep) | h << at;
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4((unsigned)w[0], (unsigned)(w[0] >> 32), (unsigned)w[1], (unsigned)(w[1] >> 32));
 }

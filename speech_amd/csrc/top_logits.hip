@@ -8,7 +8,7 @@
 // that at least k elements reach and that only k threads' elements can pass: what reaches it are the candidates, a little more
 // than k of thousands in ordinary rows, and everything below it goes straight into the log-sum-exp, relative to the bound.  The
 // candidates are ranked against each other in LDS.  Where that does not hold -- many ties, NaN, a rest that vanishes
-// beside the bound -- the workgroup finds the exact k-th key bit by bit in its registers instead (top_exact).
+// beside the bound -- the workgroup finds the exact k-th key bit by bit instead.
 #include "rows.h"
 
 namespace {
@@ -21,13 +21,25 @@ struct TopOut {
     float* rest;
 };
 
-// what a segment leaves for its row, beside its candidates
+// what a segment leaves for its row, beside `cap` candidates (0: none)
 struct TopPart {
-    int count;
     float m, s;  // the others: maximum (or any bound close above it) and the sum of exp((x - m) / T); s = 0: none
 };
 
 __device__ __forceinline__ float top_exp(float x, float m, float c) { return x == m ? 1.0f : sa_exp2((x - m) * c); }
+
+// The maximum over 1, 2 or 4 neighbouring lanes, in all of them: 256 keys a workgroup whatever its size
+template <int LANES> __device__ __forceinline__ unsigned top_group(unsigned v) {
+    if (LANES >= 2) {
+        const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false);  // quad_perm 1,0,3,2
+        v = o > v ? o : v;
+    }
+    if (LANES >= 4) {
+        const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false);  // quad_perm 2,3,0,1
+        v = o > v ? o : v;
+    }
+    return v;
+}
 
 // The largest prefix t (most significant bits first) that at least k of the 64 * N keys of this wave reach; stops where few
 // enough do.  Uniform over the wave.
@@ -59,25 +71,42 @@ template <int NT> __device__ __forceinline__ int top_count(int c, int* scratch) 
 }
 
 // Ranks the C <= kCand candidates of the block, writes the first k, leaves the values of the others in `others` in descending order
-// (the candidates themselves lie in the order of their arrival, which no result may depend on) and returns the k-th key.
+// (the candidates themselves lie in the order of their arrival, which no result may depend on) and returns the k-th key.  All
+// threads count: 128 candidates at a time, NT / 128 stretches of the list each.
+struct TopRank {
+    unsigned long long cand[kCand], kth;
+    int rank[kCand];
+    float others[kCand];
+};
 template <int NT>
-__device__ __forceinline__ unsigned long long top_rank(const unsigned long long* cand, int C, int k, long row, const TopOut& out,
-                                                       unsigned long long* kth, float* others) {
+__device__ __forceinline__ unsigned long long top_rank(TopRank& R, int C, int k, long row, const TopOut& out) {
+    constexpr int PARTS = NT / 128;
+    const int tid = threadIdx.x, part = tid >> 7;
+    for (int c = tid; c < kCand; c += NT) R.rank[c] = 0;
+    const int each = (C + PARTS - 1) / PARTS, from = part * each, to = from + each < C ? from + each : C;
     __syncthreads();
-    for (int c = threadIdx.x; c < C; c += NT) {
-        const unsigned long long key = cand[c];
+    for (int c = tid & 127; c < C; c += 128) {
+        const unsigned long long key = R.cand[c];
         int rank = 0;
-        for (int j = 0; j < C; ++j) rank += cand[j] > key;
+#pragma unroll 4
+        for (int j = from; j < to; ++j) rank += R.cand[j] > key;
+        if (rank) atomicAdd(&R.rank[c], rank);
+    }
+    __syncthreads();
+    for (int c = tid; c < C; c += NT) {
+        const unsigned long long key = R.cand[c];
+        const int rank = R.rank[c];
+        const float f = sa_unorder((unsigned)(key >> 32));
         if (rank < k) {
-            out.values[row * k + rank] = sa_unorder((unsigned)(key >> 32));
+            out.values[row * k + rank] = f;
             out.ids[row * k + rank] = (long long)(unsigned)~(unsigned)key;
-            if (rank == k - 1) *kth = key;
+            if (rank == k - 1) R.kth = key;
         } else {
-            others[rank - k] = sa_unorder((unsigned)(key >> 32));
+            R.others[rank - k] = f;
         }
     }
     __syncthreads();
-    return *kth;
+    return R.kth;
 }
 
 __device__ __forceinline__ void top_write_rest(float m, float s, float temperature, float* rest) {
@@ -86,17 +115,19 @@ __device__ __forceinline__ void top_write_rest(float m, float s, float temperatu
 
 // A segment of a row: `per` <= NT * NV vectors; nseg == 1: the whole row, and the result.  (The segments of a row are of equal
 // length: a short last one would have fewer than k threads with anything, no bound, and take the exact way.)
+// It is a chain of short phases, and what hides one is another workgroup's: registers for six waves a SIMD (4096 x 32000 bf16, k = 64:
+// 88 us; for eight, with spills, 95; unbounded 132).
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void top_segment_kernel(const T* __restrict__ x, SaRows at, int V, int k, int cap,
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void top_segment_kernel(const T* __restrict__ x, SaRows at, int V, int k, int cap,
                                                          float temperature, int nseg, int per, TopOut out,
                                                          unsigned long long* __restrict__ lists, TopPart* __restrict__ parts) {
     constexpr int VEC = SaVec<T>::N;
-    __shared__ unsigned long long cand[kCand], kth;
+    __shared__ TopRank R;
     // one key a thread, or, in rows so short that k threads might not have one, a key an element
-    constexpr int KEYS = NV == 1 ? NT * VEC : NT;
+    constexpr int KEYS = NV == 1 ? NT * VEC : 256;
     __shared__ unsigned top[KEYS], bound;
     __shared__ int count, counts[NT / 64];
-    __shared__ float sums[NT / 64], others[kCand];
+    __shared__ float sums[NT / 64];
     const long row = blockIdx.x / nseg;
     const int seg = blockIdx.x % nseg, tid = threadIdx.x;
     const T* xr = x + at.at(row);
@@ -113,6 +144,13 @@ __global__ __launch_bounds__(NT) void top_segment_kernel(const T* __restrict__ x
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, sa_element<T>(raw[i], e));
+    // (two-byte logits are widened again for every use: kept as 32 bits over the barriers they would take twice the registers)
+    auto again = [&] {
+        if constexpr (sizeof(T) == 2)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
+    };
+    again();
     if constexpr (NV == 1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
@@ -120,7 +158,8 @@ __global__ __launch_bounds__(NT) void top_segment_kernel(const T* __restrict__ x
             top[e * NT + tid] = f == f ? sa_order(f) : 0u;
         }
     } else {
-        top[tid] = sa_order(mx);
+        const unsigned u = top_group<NT / 256>(sa_order(mx));
+        if (tid % (NT / 256) == 0) top[tid / (NT / 256)] = u;
     }
     if (tid == 0) count = 0;
     __syncthreads();
@@ -133,59 +172,60 @@ __global__ __launch_bounds__(NT) void top_segment_kernel(const T* __restrict__ x
     }
     __syncthreads();
     const float b = bound <= sa_order(-INFINITY) ? -INFINITY : sa_unorder(bound);
+    // The others' sum, relative to the bound, and a bit for every element that reaches it.  (One multiply-add an element: the rounding
+    // of b c is a common factor of all terms, no more than the bound's own last place in the logarithm.)
+    constexpr int EACH = NV * VEC, WORDS = (EACH + 31) / 32, BITS = EACH < 32 ? EACH : 32;
+    const float bc = b * c;
+    unsigned hits[WORDS] = {};
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            const float f = sa_element<T>(raw[i], e);
-            if (f >= b) {
-                const int v = first + (i * NT + tid) * VEC + e;
-                if (v >= 0 && v < end) {
-                    const int p = atomicAdd(&count, 1);
-                    if (p < kCand) cand[p] = sa_rank_key(f, v);
-                }
-            } else {
-                s += sa_exp2((f - b) * c);
+            const float f = sa_element<T>(raw[i], e), u = sa_exp2(__builtin_fmaf(f, c, -bc));
+            const bool hit = f >= b;
+            s += hit ? 0.0f : u;  // (NaN stays in the sum)
+            hits[(i * VEC + e) / 32] = hits[(i * VEC + e) / 32] * 2u + (hit ? 1u : 0u);
+        }
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+        while (hits[w]) {
+            const int j = w * 32 + BITS - 32 + __builtin_clz(hits[w]);
+            hits[w] &= ~(0x80000000u >> __builtin_clz(hits[w]));
+            const int v = first + (j / VEC * NT + tid) * VEC + j % VEC;
+            if (v >= 0 && v < end) {  // (read again: it was here a moment ago)
+                const int p = atomicAdd(&count, 1);
+                if (p < kCand) R.cand[p] = sa_rank_key(sa_widen(xr[v]), v);
             }
         }
     s = sa_block_sum<NT / 64>(s, sums);
     int C = count;
     float m = b;
-    if (C > cap || (C < valid && !(s >= 0x1p-70f))) {
-        // exact: the smallest key that min(k, valid) keys reach, bit by bit
+    if (C > cap || (C < valid && !(s >= 0x1p-70f && s <= 2.0f * valid))) {
+        // exact: the smallest key that min(k, valid) keys reach, bit by bit, over the segment in memory (it was read just now)
         const int want = k < valid ? k : valid;
         unsigned long long K = 0;
         for (int bit = 63; bit >= 0; --bit) {
             const unsigned long long t = K | (1ull << bit);
             int n = 0;
-            for (int i = 0; i < NV; ++i)
-                for (int e = 0; e < VEC; ++e) {
-                    const int v = first + (i * NT + tid) * VEC + e;
-                    n += v >= 0 && v < end && sa_rank_key(sa_element<T>(raw[i], e), v) >= t;
-                }
+            for (int v = lo + tid; v < end; v += NT) n += sa_rank_key(sa_widen(xr[v]), v) >= t;
             if (top_count<NT>(n, counts) >= want) K = t;
         }
         if (tid == 0) count = 0;
         __syncthreads();
         m = -INFINITY;
-        for (int i = 0; i < NV; ++i)
-            for (int e = 0; e < VEC; ++e) {
-                const int v = first + (i * NT + tid) * VEC + e;
-                const float f = sa_element<T>(raw[i], e);
-                if (v < 0 || v >= end) continue;
-                const unsigned long long key = sa_rank_key(f, v);
-                if (key >= K) cand[atomicAdd(&count, 1)] = key;
-                else m = fmaxf(m, f);
-            }
+        for (int v = lo + tid; v < end; v += NT) {
+            const float f = sa_widen(xr[v]);
+            const unsigned long long key = sa_rank_key(f, v);
+            if (key >= K) R.cand[atomicAdd(&count, 1)] = key;
+            else m = fmaxf(m, f);
+        }
         m = sa_block_max<NT / 64>(m, sums);
         s = 0.0f;
-        for (int i = 0; i < NV; ++i)
-            for (int e = 0; e < VEC; ++e) {
-                const int v = first + (i * NT + tid) * VEC + e;
-                const float f = sa_element<T>(raw[i], e);
-                if (v >= 0 && v < end && sa_rank_key(f, v) < K) s += top_exp(f, m, c);
-            }
+        for (int v = lo + tid; v < end; v += NT) {
+            const float f = sa_widen(xr[v]);
+            if (sa_rank_key(f, v) < K) s += top_exp(f, m, c);
+        }
         s = sa_block_sum<NT / 64>(s, sums);
         C = want;
     } else if (C == valid) {
@@ -194,62 +234,61 @@ __global__ __launch_bounds__(NT) void top_segment_kernel(const T* __restrict__ x
     if (s == 0.0f) m = -INFINITY;
 
     if (nseg > 1) {
-        if (tid == 0) parts[blockIdx.x] = TopPart{C, m, s};
+        if (tid == 0) parts[blockIdx.x] = TopPart{m, s};
         __syncthreads();
-        for (int i = tid; i < C; i += NT) lists[(size_t)blockIdx.x * cap + i] = cand[i];
+        for (int i = tid; i < cap; i += NT) lists[(size_t)blockIdx.x * cap + i] = i < C ? R.cand[i] : 0;
         return;
     }
-    top_rank<NT>(cand, C, k, row, out, &kth, others);
+    top_rank<NT>(R, C, k, row, out);
     // the candidates that were not taken belong to the others
-    const float mu = C > k ? others[0] : -INFINITY;
-    const float su = sa_block_sum<NT / 64>(tid < C - k ? top_exp(others[tid], mu, c) : 0.0f, sums);
+    const float mu = C > k ? R.others[0] : -INFINITY;
+    const float su = sa_block_sum<NT / 64>(tid < C - k ? top_exp(R.others[tid], mu, c) : 0.0f, sums);
     if (tid == 0) {
         const float M = fmaxf(m, mu);
         top_write_rest(M, s * top_exp(m, M, c) + su * top_exp(mu, M, c), temperature, out.rest + row);
     }
 }
 
-// The segments of a row: the same over their candidates, which it reads where the first pass left them.
-__global__ __launch_bounds__(256) void top_merge_kernel(const unsigned long long* __restrict__ lists, const TopPart* __restrict__ parts,
-                                                        int nseg, int cap, int k, float temperature, TopOut out) {
-    constexpr int NT = 256;
-    __shared__ unsigned long long cand[kCand], kth;
-    __shared__ unsigned top[NT], bound;
+// The segments of a row: the same over their candidates, nseg * cap <= NT * EACH keys, in registers.
+template <int NT, int EACH>
+__global__ __launch_bounds__(NT) void top_merge_kernel(const unsigned long long* __restrict__ lists, const TopPart* __restrict__ parts,
+                                                       int nseg, int cap, int k, float temperature, TopOut out) {
+    __shared__ TopRank R;
+    __shared__ unsigned top[256], bound;
     __shared__ int count, counts[NT / 64];
-    __shared__ float sums[NT / 64], others[kCand];
+    __shared__ float sums[NT / 64];
     __shared__ unsigned long long total;
     __shared__ int odd;
     const long row = blockIdx.x;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, n = nseg * cap;
     const float c = SA_LOG2E / temperature;
-    lists += (size_t)row * nseg * cap;
+    lists += (size_t)row * n;
     parts += (size_t)row * nseg;
-    const int n = nseg * cap;
-    unsigned mx = 0;
-    for (int i = tid; i < n; i += NT)
-        if (i % cap < parts[i / cap].count) {
-            const unsigned u = (unsigned)(lists[i] >> 32);
-            mx = u > mx ? u : mx;
-        }
-    top[tid] = mx;
-    if (tid == 0) count = 0;
+    unsigned long long keys[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) keys[i] = i * NT + tid < n ? lists[i * NT + tid] : 0;
+    const TopPart P = tid < nseg ? parts[tid] : TopPart{-INFINITY, 0.0f};  // (nseg <= 256)
+    unsigned long long mx = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mx = keys[i] > mx ? keys[i] : mx;
+    const unsigned u = top_group<NT / 256>((unsigned)(mx >> 32));
+    if (tid % (NT / 256) == 0) top[tid / (NT / 256)] = u;
+    if (tid == 0) { count = 0; total = 0; odd = 0; }
     __syncthreads();
     if (tid < 64) {
-        unsigned key[NT / 64];
+        unsigned key[4];
 #pragma unroll
-        for (int i = 0; i < NT / 64; ++i) key[i] = top[tid + 64 * i];
+        for (int i = 0; i < 4; ++i) key[i] = top[tid + 64 * i];
         const unsigned t = top_bound(key, k);
         if (tid == 0) bound = t;
     }
     __syncthreads();
     const unsigned b = bound;
-    for (int i = tid; i < n; i += NT)
-        if (i % cap < parts[i / cap].count) {
-            const unsigned long long key = lists[i];
-            if ((unsigned)(key >> 32) >= b) {
-                const int p = atomicAdd(&count, 1);
-                if (p < kCand) cand[p] = key;
-            }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (keys[i] && (unsigned)(keys[i] >> 32) >= b) {
+            const int p = atomicAdd(&count, 1);
+            if (p < kCand) R.cand[p] = keys[i];
         }
     __syncthreads();
     int C = count;
@@ -258,74 +297,78 @@ __global__ __launch_bounds__(256) void top_merge_kernel(const unsigned long long
         for (int bit = 63; bit >= 0; --bit) {
             const unsigned long long t = K | (1ull << bit);
             int r = 0;
-            for (int i = tid; i < n; i += NT) r += i % cap < parts[i / cap].count && lists[i] >= t;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) r += keys[i] >= t;
             if (top_count<NT>(r, counts) >= k) K = t;
         }
         if (tid == 0) count = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += NT)
-            if (i % cap < parts[i / cap].count && lists[i] >= K) cand[atomicAdd(&count, 1)] = lists[i];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (keys[i] >= K) R.cand[atomicAdd(&count, 1)] = keys[i];
         C = k;
     }
-    const unsigned long long last = top_rank<NT>(cand, C, k, row, out, &kth, others);
-    float m = -INFINITY;
-    // the reference is the largest TERM, not the largest bound: a segment's sum may be as small as 2^-70 of its bound
-    for (int i = tid; i < nseg; i += NT)
-        if (parts[i].s != 0.0f) m = fmaxf(m, parts[i].m + sa_log2(parts[i].s) / c);
-    for (int i = tid; i < n; i += NT)
-        if (i % cap < parts[i / cap].count && lists[i] < last) m = fmaxf(m, sa_unorder((unsigned)(lists[i] >> 32)));
+    const unsigned long long last = top_rank<NT>(R, C, k, row, out);
+    // The others: the candidates that were not taken, and the segments' sums.  The reference is the largest TERM, not the largest
+    // bound: a segment's sum may be as small as 2^-70 of its bound.
+    float m = P.s != 0.0f ? P.m + sa_log2(P.s) / c : -INFINITY;
+    unsigned long long left = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) left = keys[i] < last && keys[i] > left ? keys[i] : left;
+    if (left) m = fmaxf(m, sa_unorder((unsigned)(left >> 32)));
     m = sa_block_max<NT / 64>(m, sums);
-    float s = 0.0f;
-    for (int i = tid; i < nseg; i += NT)
-        if (parts[i].s != 0.0f) s += parts[i].s * top_exp(parts[i].m, m, c);
-    s = sa_block_sum<NT / 64>(s, sums);
+    float s = sa_block_sum<NT / 64>(P.s != 0.0f ? P.s * top_exp(P.m, m, c) : 0.0f, sums);
     // The lists are in the order of arrival: their terms (0 .. 1) are summed as integers of 2^-32, the same in any order.
-    if (tid == 0) { total = 0; odd = 0; }
-    __syncthreads();
-    unsigned long long u = 0;
-    for (int i = tid; i < n; i += NT)
-        if (i % cap < parts[i / cap].count && lists[i] < last) {
-            const float e = top_exp(sa_unorder((unsigned)(lists[i] >> 32)), m, c);
-            if (e == e) u += (unsigned long long)(e * 0x1p32f);
-            else odd = 1;
-        }
-    if (u) atomicAdd(&total, u);
+    unsigned long long sum = 0;
+    if (left) {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (keys[i] && keys[i] < last) {
+                const float e = top_exp(sa_unorder((unsigned)(keys[i] >> 32)), m, c);
+                if (e == e) sum += (unsigned long long)(e * 0x1p32f);
+                else odd = 1;
+            }
+    }
+    if (sum) atomicAdd(&total, sum);
     __syncthreads();
     s += odd ? NAN : (float)total * 0x1p-32f;
     if (tid == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
-// Short rows (V <= 128): a wave each, every element ranked against all others.
-template <typename T>
+// Short rows (V <= 128): LANES lanes each, EACH elements a lane, every element ranked against all others.
+template <typename T, int LANES, int EACH>
 __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x, SaRows at, long rows, int V, int k,
                                                         float temperature, TopOut out) {
-    __shared__ unsigned long long keys[4][128];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long row = (long)blockIdx.x * 4 + w;
+    constexpr int ROWS = 256 / LANES;
+    __shared__ unsigned long long keys[ROWS][LANES * EACH];
+    const int lane = threadIdx.x % LANES, w = threadIdx.x / LANES;
+    const long row = (long)blockIdx.x * ROWS + w;
     if (row >= rows) return;  // (no barrier below: a wave's LDS accesses are in order)
     const T* xr = x + at.at(row);
     const float c = SA_LOG2E / temperature;
-    float f[2];
-    unsigned long long key[2];
+    float f[EACH];
+    unsigned long long key[EACH];
+    int rank[EACH];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int v = lane + 64 * i;
+    for (int i = 0; i < EACH; ++i) {
+        const int v = lane + LANES * i;
         f[i] = v < V ? sa_widen(xr[v]) : -INFINITY;
         key[i] = v < V ? sa_rank_key(f[i], v) : 0;
         keys[w][v] = key[i];
+        rank[i] = 0;
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    int rank[2] = {0, 0};
+#pragma unroll 4
     for (int j = 0; j < V; ++j) {
         const unsigned long long o = keys[w][j];
-        rank[0] += o > key[0];
-        rank[1] += o > key[1];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) rank[i] += o > key[i];
     }
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int v = lane + 64 * i;
+    for (int i = 0; i < EACH; ++i) {
+        const int v = lane + LANES * i;
         if (v >= V) continue;
         if (rank[i] < k) {
             out.values[row * k + rank[i]] = f[i];
@@ -334,26 +377,35 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x,
             m = fmaxf(m, f[i]);
         }
     }
-    m = sa_wave_max(m);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, LANES));
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < V && rank[i] >= k) s += top_exp(f[i], m, c);
-    s = sa_wave_sum(s);
+    for (int i = 0; i < EACH; ++i)
+        if (lane + LANES * i < V && rank[i] >= k) s += top_exp(f[i], m, c);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, LANES);
     if (lane == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
+// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88 us
+// whole, 90 + 23 in two segments and a merge); others are split into segments of 256 threads, shorter ones where there are few rows, as long as one workgroup can hold what the segments leave.
 struct TopPlan {
-    int nv, nseg, per, cap;  // vectors a thread, segments a row, vectors a segment, candidates a segment may leave
+    int nt, nv, nseg, per, cap;  // threads, vectors a thread, segments a row, vectors a segment, candidates a segment leaves
 };
-TopPlan top_plan(int V, int k, int dtype) {
+TopPlan top_plan(long rows, int V, int k, int dtype) {
     const int vec = dtype == SA_F32 ? 4 : 8, vectors = (V + vec - 1 + vec - 1) / vec;  // the longest row, with its lead
-    TopPlan p;
-    p.nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : vectors <= 1024 ? 4 : 8;
-    p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
-    p.per = (vectors + p.nseg - 1) / p.nseg;
-    p.nseg = (vectors + p.per - 1) / p.per;
-    p.cap = k + k / 2 + 32;
+    TopPlan p{256, 8, 1, vectors, k + k / 2 + 32};
+    if (vectors <= 256 * 8) {
+        p.nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : vectors <= 1024 ? 4 : 8;
+    } else if (vectors <= 1024 * 8 && rows >= 256) {
+        p.nt = vectors <= 512 * 8 ? 512 : 1024;
+    } else {
+        if (rows * ((vectors + 2047) / 2048) < 128 && (vectors + 1023) / 1024 * p.cap <= 16384) p.nv = 4;
+        p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
+        p.per = (vectors + p.nseg - 1) / p.nseg;
+        p.nseg = (vectors + p.per - 1) / p.per;
+    }
     return p;
 }
 size_t top_bytes(long rows, const TopPlan& p) {
@@ -367,36 +419,48 @@ void top_launch(const void* x, const SaRows& at, long rows, int V, int k, float 
                 const TopPlan& p, char* ws, hipStream_t stream) {
     const T* xt = (const T*)x;
     if (V <= 128) {
-        hipLaunchKernelGGL((top_short_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, xt, at, rows, V, k,
-                           temperature, out);
+#define TOP_SHORT(LANES, EACH)                                                                                             \
+    hipLaunchKernelGGL((top_short_kernel<T, LANES, EACH>), dim3((unsigned)((rows * LANES + 255) / 256)), dim3(256), 0, stream, xt, \
+                       at, rows, V, k, temperature, out)
+        if (V <= 32) TOP_SHORT(32, 1);
+        else if (V <= 64) TOP_SHORT(64, 1);
+        else TOP_SHORT(64, 2);
+#undef TOP_SHORT
         return;
     }
     TopPart* parts = (TopPart*)ws;
     unsigned long long* lists = (unsigned long long*)(ws + sa_align_up((size_t)rows * p.nseg * sizeof(TopPart), 256));
-    const int cap = p.nseg == 1 ? kCand : p.cap;
-    const dim3 grid((unsigned)(rows * p.nseg)), block(256);
-#define TOP_LAUNCH(NV)                                                                                                     \
-    hipLaunchKernelGGL((top_segment_kernel<T, 256, NV>), grid, block, 0, stream, xt, at, V, k, cap, temperature, p.nseg, p.per, out, \
+    const int cap = p.nseg == 1 ? kCand : p.cap, n = p.nseg * p.cap;
+    const dim3 grid((unsigned)(rows * p.nseg)), block(p.nt);
+#define TOP_LAUNCH(NT, NV)                                                                                                   \
+    hipLaunchKernelGGL((top_segment_kernel<T, NT, NV>), grid, block, 0, stream, xt, at, V, k, cap, temperature, p.nseg, p.per, out, \
                        lists, parts)
-    if (p.nv == 1) TOP_LAUNCH(1);
-    else if (p.nv == 2) TOP_LAUNCH(2);
-    else if (p.nv == 4) TOP_LAUNCH(4);
-    else TOP_LAUNCH(8);
+    if (p.nt == 1024) TOP_LAUNCH(1024, 8);
+    else if (p.nt == 512) TOP_LAUNCH(512, 8);
+    else if (p.nv == 1) TOP_LAUNCH(256, 1);
+    else if (p.nv == 2) TOP_LAUNCH(256, 2);
+    else if (p.nv == 4) TOP_LAUNCH(256, 4);
+    else TOP_LAUNCH(256, 8);
 #undef TOP_LAUNCH
-    if (p.nseg > 1)
-        hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)rows), dim3(256), 0, stream, (const unsigned long long*)lists,
-                           (const TopPart*)parts, p.nseg, p.cap, k, temperature, out);
+    if (p.nseg == 1) return;
+#define TOP_MERGE(NT, EACH)                                                                                            \
+    hipLaunchKernelGGL((top_merge_kernel<NT, EACH>), dim3((unsigned)rows), dim3(NT), 0, stream, (const unsigned long long*)lists, \
+                       (const TopPart*)parts, p.nseg, p.cap, k, temperature, out)
+    if (n <= 256 * 8) TOP_MERGE(256, 8);
+    else if (n <= 1024 * 8) TOP_MERGE(1024, 8);
+    else TOP_MERGE(1024, 32);  // (129 segments of 224 at most: 28896 keys)
+#undef TOP_MERGE
 }
 
 bool top_ok(long rows, int V, int k, int dtype) {
     return rows >= 0 && sa_rows_ok(dtype, V) && k >= 1 && k <= V && k <= SA_TOP_MAX &&
-           (size_t)rows * (size_t)top_plan(V, k, dtype).nseg <= 0x7fffffffu;
+           (size_t)rows * (size_t)top_plan(rows, V, k, dtype).nseg <= 0x7fffffffu;
 }
 
 }  // namespace
 
 extern "C" size_t sa_top_logits_workspace_bytes(long rows, int V, int k, int dtype) {
-    return top_ok(rows, V, k, dtype) ? top_bytes(rows, top_plan(V, k, dtype)) : 0;
+    return top_ok(rows, V, k, dtype) ? top_bytes(rows, top_plan(rows, V, k, dtype)) : 0;
 }
 
 extern "C" ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner, int n_inner, int dtype, long rows, int V,
@@ -406,7 +470,7 @@ extern "C" ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner
     if (!top_ok(rows, V, k, dtype) || n_inner < 1 || !(temperature > 0.f) || !(temperature < INFINITY))
         return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
-    const TopPlan p = top_plan(V, k, dtype);
+    const TopPlan p = top_plan(rows, V, k, dtype);
     if (!x || !values || !ids || !rest || (top_bytes(rows, p) && (!workspace || workspace_bytes < top_bytes(rows, p))))
         return CTC_STATUS_INVALID_VALUE;
     const SaRows at{ld_outer, ld_inner, n_inner};
