@@ -602,6 +602,17 @@ size_t sa_logits_pick_workspace_bytes(int rows, int V, int dtype);
 ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int rows, int V, const saConstraints* c,
                            long long* d_tokens, float* d_logp, void* workspace, size_t workspace_bytes, void* stream);
 
+/* sa_s2s_greedy_decode (section 8) with constraints on every token: K logits per request as above; c's own history, lengths and
+ * states are not read.  penalties != 0: the history of request b is its row of d_tokens so far (the start token is no class).
+ * d_states (rows) int, with a mask: the request's mask row, moved on to d_next_states[state * K + token] ((n_states, K) int, or
+ * NULL: it stays) after every token; a state outside the mask is unmasked from then on.  A request that has no token left emits
+ * end_tok.  max_len < SA_LIST_MAX; workspace: sa_s2s_greedy_workspace_bytes. */
+ctcStatus_t sa_s2s_greedy_decode_constrained(const float* eh, const float* const* params, int B, int T, int H, int E, int KS,
+                                             int K, float scale, int end_tok, int max_len, int check_every,
+                                             const saConstraints* c, int penalties, int* d_states, const int* d_next_states,
+                                             long long* d_tokens, int* d_steps, void* workspace, size_t workspace_bytes,
+                                             void* stream);
+
 /* The k largest logits of every row (k <= V, k <= SA_TOP_MAX) in descending order, ties to the lowest index, NaN above
  * everything: values (rows, k) float, ids (rows, k) int64, and rest[row] = log sum exp(x_v / temperature) over the OTHER V - k
  * tokens (-inf when there are none) -- what a distillation loss needs of a teacher's row.

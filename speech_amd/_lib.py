@@ -150,6 +150,8 @@ SIGNATURES = {
                                                                                                   c_void_p, c_size_t, c_void_p]),
     "sa_softmax_xent": (c_int, [c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_long, c_int, c_void_p]),
     "sa_argmax_rows": (c_int, [c_void_p, c_void_p, c_long, c_int, c_void_p]),
+    "sa_s2s_greedy_decode_constrained": (c_int, [c_void_p, c_void_p] + [c_int] * 6 + [c_float] + [c_int] * 3 +
+                                         [ctypes.POINTER(saConstraints), c_int] + [c_void_p] * 5 + [c_size_t, c_void_p]),
     "sa_logits_constrain": (c_int, [c_void_p, c_long, c_int, c_void_p, c_long, c_int, c_int,
                                     ctypes.POINTER(saConstraints), c_void_p]),
     "sa_logits_pick_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),

@@ -1806,12 +1806,19 @@ extern "C" ctcStatus_t sa_s2s_beam_search(const float* eh, const float* const* p
 namespace {
 
 struct GreedyState { int done, steps; };
+struct GreedyGrammar {  // constrained decode: on; where each request's grammar goes after a token (next: (n_states, K), or none)
+    int on;
+    int* states;
+    const int* next;
+    int n_states;
+};
 
 __global__ __launch_bounds__(64) void s2s_greedy_pick_kernel(GreedyState* st, const float* __restrict__ logits,
                                                             long long* __restrict__ tokens, long long* __restrict__ idx,
                                                             unsigned* __restrict__ count, int B, int K, int ncol, int step,
                                                             int end_tok, int max_len, const float* __restrict__ emb,
-                                                            const float* __restrict__ sx, float* __restrict__ ix, int E) {
+                                                            const float* __restrict__ sx, float* __restrict__ ix, int E,
+                                                            GreedyGrammar G) {
     if (st->done) return;
     const int b = blockIdx.x, lane = threadIdx.x;
     const float* xr = logits + (long)b * K;
@@ -1825,6 +1832,18 @@ __global__ __launch_bounds__(64) void s2s_greedy_pick_kernel(GreedyState* st, co
         const int oi = __shfl_xor(bi, o, 64);
         if (ob > best || (ob == best && oi < bi)) { best = ob; bi = oi; }
     }
+    if (G.on && best == -3.0e38f) {  // constrained: where nothing is left, the request ends; a value below -3e38 is still a value
+        float any = -INFINITY;
+        for (int k = lane; k < K; k += 64)
+            if (xr[k] > any) { any = xr[k]; bi = k; }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const float ob = __shfl_xor(any, o, 64);
+            const int oi = __shfl_xor(bi, o, 64);
+            if (ob > any || (ob == any && oi < bi)) { any = ob; bi = oi; }
+        }
+        if (any == -INFINITY) bi = end_tok;
+    }
     // a row without a finite maximum (all NaN / all -inf: nothing ever compared greater) picks class 0, a valid index
     // like the one torch.max returns there, rather than reading the embedding 2^31 rows out of bounds
     if ((unsigned)bi >= (unsigned)K) bi = 0;
@@ -1832,6 +1851,10 @@ __global__ __launch_bounds__(64) void s2s_greedy_pick_kernel(GreedyState* st, co
     if (lane == 0) {
         tokens[(long)b * ncol + step + 1] = bi;
         idx[b] = bi;
+        if (G.next) {
+            const int state = G.states[b];
+            if (state >= 0 && state < G.n_states) G.states[b] = G.next[(long)state * K + bi];
+        }
         // the last row to arrive closes the step: count[step] = rows done, high half = rows that emitted the end token
         const unsigned add = 1u + (bi == end_tok ? 0x10000u : 0u);
         const unsigned seen = atomicAdd(&count[step], add) + add;
@@ -1876,10 +1899,11 @@ extern "C" size_t sa_s2s_greedy_workspace_bytes(int B, int T, int H, int E, int 
     return greedy_layout(B, T, H, E, K, max_len).total;
 }
 
-extern "C" ctcStatus_t sa_s2s_greedy_decode(const float* eh, const float* const* params, int B, int T, int H, int E, int KS,
-                                            int K, float scale, int end_tok, int max_len, int check_every,
-                                            long long* d_tokens, int* d_steps, void* workspace, size_t workspace_bytes,
-                                            void* stream_) {
+namespace {
+// c == NULL: the plain decode; states: B ints of the caller's that the decode moves on (the requests' grammar states)
+ctcStatus_t greedy_run(const float* eh, const float* const* params, int B, int T, int H, int E, int KS, int K, float scale,
+                       int end_tok, int max_len, int check_every, const saConstraints* c, int* states, const int* next,
+                       long long* d_tokens, int* d_steps, void* workspace, size_t workspace_bytes, void* stream_) {
     SA_CLEAR_ERR();
     S2SDims d{B, T, 1, H, E, KS, K};
     if (!eh || !params || !d_tokens || !d_steps || !workspace || !s2s_ok(d) || max_len < 1 || B > 65535 || check_every < 0)
@@ -1899,6 +1923,14 @@ extern "C" ctcStatus_t sa_s2s_greedy_decode(const float* eh, const float* const*
     float* score = (float*)(ws + L.score);
     const float* const* P = params;
     const int ncol = max_len + 1;
+    saConstraints con;
+    if (c) {
+        con = *c;
+        con.lengths = nullptr;
+        con.history_ld = ncol;
+        con.states = states;
+    }
+    const GreedyGrammar grammar{c != nullptr, states, c ? next : nullptr, c ? c->n_states : 0};
     const size_t smem1 = ((size_t)(kAttTB + KS - 1) + (size_t)H * KS + (size_t)H) * sizeof(float);
     const size_t smem2 = ((size_t)T + 8 + 4 * (size_t)H) * sizeof(float);
     if (!att_smem((const void*)attention_score_kernel, smem1) || !att_smem((const void*)attention_context_kernel, smem2))
@@ -1925,8 +1957,14 @@ extern "C" ctcStatus_t sa_s2s_greedy_decode(const float* eh, const float* const*
         context_launch(A, score, ax, sx, oin, B, smem2, stream);
         SkinnyProb q{oin, P[P_FCW], P[P_FCB], logits, K, H, 0, H, H, K};
         skinny_launch(&q, 1, B, stream);
+        if (c) {  // in place; the tokens so far are the history of the penalties
+            con.history = c->history_len ? d_tokens : nullptr;
+            con.history_len = c->history_len ? t + 1 : 0;
+            const ctcStatus_t r = sa_logits_constrain(logits, K, SA_F32, logits, K, B, K, &con, stream_);
+            if (r != CTC_STATUS_SUCCESS) return r;
+        }
         hipLaunchKernelGGL(s2s_greedy_pick_kernel, dim3(B), dim3(64), 0, stream, st, (const float*)logits, d_tokens, idx, count, B,
-                           K, ncol, t, end_tok, max_len, P[P_EMB], (const float*)sx, ix, E);
+                           K, ncol, t, end_tok, max_len, P[P_EMB], (const float*)sx, ix, E, grammar);
         if (check_every > 0 && (t + 1) % check_every == 0 && t + 1 < max_len) {
             int done = 0;
             if (hipMemcpyAsync(&done, &st->done, sizeof(int), hipMemcpyDeviceToHost, stream) != hipSuccess ||
@@ -1939,4 +1977,27 @@ extern "C" ctcStatus_t sa_s2s_greedy_decode(const float* eh, const float* const*
         return CTC_STATUS_MEMOPS_FAILED;
     SA_CHECK_LAUNCH();
     return CTC_STATUS_SUCCESS;
+}
+}  // namespace
+
+extern "C" ctcStatus_t sa_s2s_greedy_decode(const float* eh, const float* const* params, int B, int T, int H, int E, int KS,
+                                            int K, float scale, int end_tok, int max_len, int check_every,
+                                            long long* d_tokens, int* d_steps, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+    return greedy_run(eh, params, B, T, H, E, KS, K, scale, end_tok, max_len, check_every, nullptr, nullptr, nullptr, d_tokens,
+                      d_steps, workspace, workspace_bytes, stream);
+}
+
+extern "C" ctcStatus_t sa_s2s_greedy_decode_constrained(const float* eh, const float* const* params, int B, int T, int H, int E,
+                                                        int KS, int K, float scale, int end_tok, int max_len, int check_every,
+                                                        const saConstraints* c, int penalties, int* d_states,
+                                                        const int* d_next_states, long long* d_tokens, int* d_steps,
+                                                        void* workspace, size_t workspace_bytes, void* stream) {
+    if (!c || max_len >= SA_LIST_MAX || end_tok < 0 || end_tok >= K || (c->mask && !d_states) || (d_next_states && !c->mask))
+        return CTC_STATUS_INVALID_VALUE;
+    saConstraints con = *c;
+    con.history = nullptr;
+    con.history_len = penalties ? 1 : 0;
+    return greedy_run(eh, params, B, T, H, E, KS, K, scale, end_tok, max_len, check_every, &con, con.mask ? d_states : nullptr,
+                      d_next_states, d_tokens, d_steps, workspace, workspace_bytes, stream);
 }

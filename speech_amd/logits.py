@@ -114,7 +114,8 @@ def _penalty(value, name, rows, device, neutral):
     return None, value
 
 
-def _constraints(rows, V, dev, history, lengths, repetition, presence, frequency, bias_ids, bias_values, mask, states):
+def _constraints(rows, V, dev, history, lengths, repetition, presence, frequency, bias_ids, bias_values, mask, states, decoding=False):
+    """The arguments of `constrain`, checked, as the library reads them.  decoding: the decode itself keeps the history."""
     c = _lib.saConstraints()
     if history is not None:
         c.history, c.history_ld, c.history_len = _list(history, "history", rows, dev, torch.int64)
@@ -125,7 +126,7 @@ def _constraints(rows, V, dev, history, lengths, repetition, presence, frequency
     c.repetition, c.repetition_all = _penalty(repetition, "repetition", rows, dev, 1.0)
     c.presence, c.presence_all = _penalty(presence, "presence", rows, dev, 0.0)
     c.frequency, c.frequency_all = _penalty(frequency, "frequency", rows, dev, 0.0)
-    if history is None and not (repetition is None and presence is None and frequency is None):
+    if history is None and not decoding and not (repetition is None and presence is None and frequency is None):
         raise SpeechAmdError("penalties for repeated tokens need a history")
     if (bias_ids is None) != (bias_values is None):
         raise SpeechAmdError("bias_ids and bias_values come together")
@@ -151,6 +152,26 @@ def _constraints(rows, V, dev, history, lengths, repetition, presence, frequency
     elif states is not None:
         raise SpeechAmdError("states without a mask")
     return c
+
+
+def decoding_constraints(rows, V, dev, repetition=None, presence=None, frequency=None, bias_ids=None, bias_values=None,
+                         mask=None, states=None, next_states=None):
+    """What a constrained decode takes (Seq2Seq.infer(constraints=...)): the arguments of `constrain` without a history -- the
+    tokens of the decode are that --, and the grammar's transitions: after token v a request in state s goes on in
+    next_states[s, v] ((states, V) int32; it stays without them).  Requests start in `states`, or all in state 0; a state
+    outside the mask is unmasked from then on.  Returns (saConstraints, penalties, states, pointer of next_states)."""
+    if mask is not None and states is None:
+        states = torch.zeros(rows, dtype=torch.int32, device=dev)
+    c = _constraints(rows, V, dev, None, None, repetition, presence, frequency, bias_ids, bias_values, mask, states, decoding=True)
+    following = None
+    if next_states is not None:
+        if mask is None:
+            raise SpeechAmdError("next_states without a mask")
+        following = _tensor(next_states, "next_states", torch.int32, (mask.shape[0], V), dev)
+    penalties = not (repetition is None and presence is None and frequency is None)
+    if states is not None:
+        states = states.clone()  # the decode moves its own copy on
+    return c, penalties, states, following
 
 
 def _matrix(logits):

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from . import _lib, ctc, decoder, seq2seq as _s2s, transducer as _tr
+from . import _lib, ctc, decoder, logits as _logits, seq2seq as _s2s, transducer as _tr
 from .encoder import EncoderFunction, EncoderPlan
 
 
@@ -639,6 +639,29 @@ class Seq2Seq(Model):
             # sum / batch_size (:61-63); a data-parallel shard divides by the GLOBAL batch size
             return _s2s.XentFunction.apply(out, tgt, 1.0 / (self.loss_denominator or batch_size))
 
+    def top_logits(self, batch, k, temperature=1.0):
+        """What this model, as a teacher, leaves of a batch for distill_loss: (values (B, U-1, k), ids (B, U-1, k), rest (B, U-1)),
+        the k largest logits of every output token and the log-sum-exp of the others (speech_amd.logits.top_logits)."""
+        def run():
+            with torch.no_grad():
+                out = _logits.top_logits(self(batch), k, temperature)
+            torch.cuda.current_stream().synchronize()
+            return out
+        return self._healthy(run)
+
+    def distill_loss(self, batch, values, ids, rest=None, weights=None, temperature=1.0, alpha=1.0):
+        """The loss of this model, as a student, on a teacher's top logits: alpha T^2 KL + (1 - alpha) cross-entropy
+        (speech_amd.logits.DistillLoss), summed over the tokens and divided by the batch size like loss() -- which it is at
+        alpha = 0.  `weights` (B, U-1) leaves padded tokens out (0); the reference scores them."""
+        x, y = self._collate_staged(*batch)
+        if self.is_cuda:
+            x = self._to_device(x)
+            y = y.cuda(non_blocking=True)
+        with torch.set_grad_enabled(not self.volatile):
+            out, _ = self.forward_impl(x, y)
+            loss_fn = _logits.DistillLoss(temperature, alpha, denom=self.loss_denominator or out.shape[0])
+            return loss_fn(out, values, ids, rest=rest, targets=y[:, 1:].contiguous(), weights=weights)
+
     def forward_impl(self, x, y):
         x = self.encode(x)
         return self.decode(x, y)
@@ -683,8 +706,11 @@ class Seq2Seq(Model):
                 break
         return torch.cat(probs), torch.cat(argmaxs, dim=1)
 
-    def infer(self, batch, max_len=200):
-        """seq2seq.py:160-178: greedy decode from the start tokens (no beam search)."""
+    def infer(self, batch, max_len=200, constraints=None):
+        """seq2seq.py:160-178: greedy decode from the start tokens (no beam search).
+        constraints: penalties for repeated tokens, biases and a grammar that every token is held to, a dict of
+        speech_amd.logits.decoding_constraints' arguments (requests = utterances, V = vocab_size - 1 classes); an utterance
+        that has no token left emits the end token."""
         x, y = self._collate_staged(*batch)
         end_tok = int(y[0, -1])
 
@@ -693,7 +719,8 @@ class Seq2Seq(Model):
                 enc = self.encode(self._to_device(x))
                 # the whole token loop in the library (no device -> host round trip per token); infer_decode remains the
                 # step-by-step form of the reference's API
-                toks = _s2s.greedy_decode(enc, y[:, 0], self._param_dict(), self.attend.log_t, end_tok, max_len)
+                toks = _s2s.greedy_decode(enc, y[:, 0], self._param_dict(), self.attend.log_t, end_tok, max_len,
+                                          constraints=constraints)
             return [seq.tolist() for seq in toks.numpy()]
         return self._healthy(run)
 

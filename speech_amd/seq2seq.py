@@ -15,7 +15,7 @@ import random
 
 import torch
 
-from . import _lib, ops
+from . import _lib, logits, ops
 
 
 def _L():
@@ -102,9 +102,10 @@ def step(eh, idx, state, P, log_t):
     return out, (hx, ax, sx)
 
 
-def greedy_decode(eh, y0, P, log_t, end_tok, max_len, check_every=8):
+def greedy_decode(eh, y0, P, log_t, end_tok, max_len, check_every=8, constraints=None):
     """Seq2Seq.infer_decode's token matrix (seq2seq.py:140-158) for a batch, the whole loop in the library
-    (sa_s2s_greedy_decode): eh (B, T, H), y0 (B,) start tokens.  Returns an int64 CPU tensor (B, steps + 1)."""
+    (sa_s2s_greedy_decode): eh (B, T, H), y0 (B,) start tokens.  Returns an int64 CPU tensor (B, steps + 1).
+    constraints: a dict of logits.decoding_constraints' arguments (sa_s2s_greedy_decode_constrained)."""
     B, T, H = eh.shape
     E, K, KS = P["emb"].shape[1], P["fc_w"].shape[0], P["conv_w"].shape[-1]
     L = _L()
@@ -116,10 +117,18 @@ def greedy_decode(eh, y0, P, log_t, end_tok, max_len, check_every=8):
     tokens = rec[:B * (max_len + 1)].view(B, max_len + 1)
     tokens[:, 0] = y0.reshape(-1).to(eh.device)
     plist = [P[n].contiguous() for n in _NAMES]
-    _lib.check(L.sa_s2s_greedy_decode(_lib.ptr(eh.contiguous()), _ptr_array(plist), B, T, H, E, KS, K,
-                                      math.log(T) if log_t else 1.0, int(end_tok), int(max_len), int(check_every),
-                                      tokens.data_ptr(), rec.data_ptr() + 8 * B * (max_len + 1), _lib.ptr(ws), ws.numel(),
-                                      _lib.cur_stream()), "sa_s2s_greedy_decode")
+    if constraints is not None:
+        con, penalties, states, following = logits.decoding_constraints(B, K, eh.device, **constraints)
+        _lib.check(L.sa_s2s_greedy_decode_constrained(
+            _lib.ptr(eh.contiguous()), _ptr_array(plist), B, T, H, E, KS, K, math.log(T) if log_t else 1.0, int(end_tok),
+            int(max_len), int(check_every), ctypes.byref(con), int(penalties), _lib.ptr(states), following, tokens.data_ptr(),
+            rec.data_ptr() + 8 * B * (max_len + 1), _lib.ptr(ws), ws.numel(), _lib.cur_stream()),
+            "sa_s2s_greedy_decode_constrained")
+    else:
+        _lib.check(L.sa_s2s_greedy_decode(_lib.ptr(eh.contiguous()), _ptr_array(plist), B, T, H, E, KS, K,
+                                          math.log(T) if log_t else 1.0, int(end_tok), int(max_len), int(check_every),
+                                          tokens.data_ptr(), rec.data_ptr() + 8 * B * (max_len + 1), _lib.ptr(ws), ws.numel(),
+                                          _lib.cur_stream()), "sa_s2s_greedy_decode")
     host = rec.cpu()
     steps = int(host[-1:].numpy().view("int32")[0])
     return host[:B * (max_len + 1)].view(B, max_len + 1)[:, :steps + 1]
