@@ -11,10 +11,33 @@
 
 namespace {
 
-struct PickPart {  // what a segment leaves for its row: the best token, the maximum and the sum of exp(x - maximum)
-    unsigned long long key;
+// What a wave leaves for its segment, and a segment for its row: the order of the best value (sa_order: NaN above all) and the
+// lowest token that has it, the largest number and the sum of exp(x - m).  m = -inf: no numbers.
+struct PickPart {
+    unsigned best;
+    int token;
     float m, s;
 };
+__device__ __forceinline__ void pick_better(PickPart& a, unsigned best, int token) {
+    if (best > a.best || (best == a.best && token < a.token)) { a.best = best; a.token = token; }
+}
+__device__ __forceinline__ void pick_write(const PickPart& a, long long* token, float* logp) {
+    const bool none = a.best <= sa_order(-INFINITY);
+    *token = none ? -1 : a.token;
+    *logp = none ? -INFINITY : -logf(a.s);
+}
+// the smallest of the lanes' numbers, in all of them
+__device__ __forceinline__ int con_wave_min(int v) {
+#define CON_DPP_MIN(ctrl, rows)                                                          \
+    {                                                                                    \
+        const int o = __builtin_amdgcn_update_dpp(v, v, (ctrl), (rows), 0xf, false);     \
+        v = o < v ? o : v;                                                               \
+    }
+    CON_DPP_MIN(0x111, 0xf) CON_DPP_MIN(0x112, 0xf) CON_DPP_MIN(0x114, 0xf) CON_DPP_MIN(0x118, 0xf)  // row_shr 1, 2, 4, 8
+    CON_DPP_MIN(0x142, 0xa) CON_DPP_MIN(0x143, 0xc)                                                  // row_bcast 15, 31
+#undef CON_DPP_MIN
+    return __builtin_amdgcn_readlane(v, 63);
+}
 
 // exp(x - m) where equal infinities count as equal (a bias of +inf forces its token)
 __device__ __forceinline__ float con_exp(float x, float m) { return x == m ? 1.0f : sa_exp2((x - m) * SA_LOG2E); }
@@ -44,13 +67,23 @@ __global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T*
                                                         saConstraints C, PickPart* __restrict__ part, long long* __restrict__ tokens,
                                                         float* __restrict__ logp) {
     constexpr int VEC = SaVec<T>::N, NT = 256, SEG = NT * NV * VEC;
-    extern __shared__ unsigned words[];  // SEG words, then SEG positions (16 bits); nothing where there are no lists
+    extern __shared__ uint4 words4[];  // SEG words, then SEG positions (16 bits); nothing where there are no lists
     __shared__ int found;
-    __shared__ float scratch[NT / 64];
-    __shared__ unsigned long long best[NT / 64];
+    __shared__ PickPart waves[NT / 64];
+    unsigned* const words = (unsigned*)words4;
     const int row = blockIdx.x / nseg, seg = blockIdx.x % nseg, tid = threadIdx.x;
     const T* xr = x + (long)row * ldx;
     const int first = seg * per * VEC - sa_lead(xr), end = first + per * VEC < V ? first + per * VEC : V;
+    // Everything the row needs from memory is asked for at once, the lists first: their atomics are the longer way.
+    const bool lists = C.history || C.bias_ids;
+    constexpr int AHEAD = 8;  // history entries a thread has in flight (2048 a workgroup)
+    long long past[AHEAD], biased = -1;
+    const long long* h = C.history + (long)row * C.history_ld;
+    const long long* ids = C.bias_ids + (long)row * C.bias_ld;
+    if (C.history)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) past[u] = u * NT + tid < C.history_len ? h[u * NT + tid] : -1;
+    if (C.bias_ids && tid < C.n_bias) biased = ids[tid];
     uint4 raw[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, first + (i * NT + tid) * VEC, end);
@@ -59,7 +92,12 @@ __global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T*
         const int state = C.states ? C.states[row] : row;
         if (state >= 0 && state < C.n_states) mask = C.mask + (long)state * C.mask_ld;
     }
-    const bool lists = C.history || C.bias_ids;
+    unsigned allowed[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v0 = first + (i * NT + tid) * VEC;
+        allowed[i] = mask && v0 < end ? con_allowed<VEC>(mask, v0, V) : ~0u;
+    }
     if (lists) {
         sa_u16* places = (sa_u16*)(words + SEG);
         const float r = C.repetition ? C.repetition[row] : C.repetition_all;
@@ -71,30 +109,35 @@ __global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T*
             len = C.lengths ? C.lengths[row] : C.history_len;
             len = len < 0 ? 0 : (len > C.history_len ? C.history_len : len);
         }
-        uint4* clear = (uint4*)words;
 #pragma unroll
-        for (int i = 0; i < SEG / 4 / NT; ++i) clear[i * NT + tid] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < SEG / 4 / NT; ++i) words4[i * NT + tid] = make_uint4(0, 0, 0, 0);
         if (tid == 0) found = 0;
         // (a token t of a list is the segment's when `first` <= t < `end`; t >= 0 keeps what lies before the row out; the last
         // segment of a row that starts on a boundary may be empty, and begin behind the row's end)
         const unsigned long long n = end > first ? (unsigned long long)(end - first) : 0ull;
+        auto add_bias = [&](long long t, int j) {
+            const unsigned long long d = (unsigned long long)(t - first);
+            if (t >= 0 && d < n && atomicMax(&words[d], (unsigned)(j + 1) << 16) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
+        };
+        auto add_past = [&](long long t) {
+            const unsigned long long d = (unsigned long long)(t - first);
+            if (t >= 0 && d < n && atomicAdd(&words[d], 1u) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
+        };
         __syncthreads();
         if (C.bias_ids) {
-            const long long* ids = C.bias_ids + (long)row * C.bias_ld;
-            for (int j = tid; j < C.n_bias; j += NT) {
-                const long long t = ids[j];
-                const unsigned long long d = (unsigned long long)(t - first);
-                if (t >= 0 && d < n && atomicMax(&words[d], (unsigned)(j + 1) << 16) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
-            }
+            if (tid < C.n_bias) add_bias(biased, tid);
+            for (int j = NT + tid; j < C.n_bias; j += NT) add_bias(ids[j], j);
             __syncthreads();
         }
         if (len > 0) {
-            const long long* h = C.history + (long)row * C.history_ld;
-#pragma unroll 4
-            for (int i = tid; i < len; i += NT) {
-                const long long t = h[i];
-                const unsigned long long d = (unsigned long long)(t - first);
-                if (t >= 0 && d < n && atomicAdd(&words[d], 1u) == 0) places[atomicAdd(&found, 1)] = (sa_u16)d;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (u * NT + tid < len) add_past(past[u]);
+            for (int i = AHEAD * NT; i < len; i += AHEAD * NT) {
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) past[u] = i + u * NT + tid < len ? h[i + u * NT + tid] : -1;
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) add_past(past[u]);
             }
         }
         __syncthreads();
@@ -107,109 +150,100 @@ __global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T*
     }
     T* yr = PICK ? nullptr : y + (long)row * ldy;
     const bool aligned = !PICK && sa_lead(yr) == sa_lead(xr);
-    unsigned long long key = 0;
-    float m = -INFINITY, val[PICK ? NV * VEC : VEC];
+    float val[PICK ? NV * VEC : VEC], top = -INFINITY;
+    int token = 0x7fffffff;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int q = i * NT + tid, v0 = first + q * VEC;
-        if (v0 >= end) {
-            if (PICK)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) val[i * VEC + e] = -INFINITY;
-            continue;
-        }
         float* g = val + (PICK ? i * VEC : 0);
-        const unsigned allowed = mask ? con_allowed<VEC>(mask, v0, V) : ~0u;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            g[e] = sa_element<T>(raw[i], e);
-            if (lists) {
-                const unsigned w = words[q * VEC + e];
-                g[e] = w ? __builtin_bit_cast(float, w) : g[e];
+        for (int e = 0; e < VEC; ++e) g[e] = sa_element<T>(raw[i], e);
+        if (lists) {
+#pragma unroll
+            for (int e = 0; e < VEC; e += 4) {
+                const uint4 w = words4[(q * VEC + e) / 4];
+                g[e] = w.x ? __builtin_bit_cast(float, w.x) : g[e];
+                g[e + 1] = w.y ? __builtin_bit_cast(float, w.y) : g[e + 1];
+                g[e + 2] = w.z ? __builtin_bit_cast(float, w.z) : g[e + 2];
+                g[e + 3] = w.w ? __builtin_bit_cast(float, w.w) : g[e + 3];
             }
-            g[e] = (allowed >> e) & 1u ? g[e] : -INFINITY;
         }
-        if constexpr (PICK) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (v0 + e >= 0 && v0 + e < end) {
-                    const unsigned long long k = sa_rank_key(g[e], v0 + e);
-                    key = k > key ? k : key;
-                    m = fmaxf(m, g[e]);
-                } else {
-                    g[e] = -INFINITY;
-                }
-            }
-        } else {
+        for (int e = 0; e < VEC; ++e) g[e] = (allowed[i] >> e) & 1u ? g[e] : -INFINITY;
+        if constexpr (PICK) {  // (what lies outside the row was loaded as -inf and is in no list)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (g[e] > top) { top = g[e]; token = v0 + e; }
+        } else if (v0 < end) {
             sa_store_vec<T>(yr, v0, end, g, aligned);
         }
     }
     if constexpr (PICK) {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor(key, o, 64);
-            key = other > key ? other : key;
-        }
-        if ((tid & 63) == 0) best[tid >> 6] = key;
-        m = sa_block_max<NT / 64>(m, scratch);  // (its barriers also publish `best`)
+        const int lane = tid & 63;
+        const float m = sa_wave_max_dpp(top), b = m > -INFINITY ? m : 0.0f;
         float s = 0.0f;
-        if (m > -INFINITY) {  // (else every exponential would be that of equal infinities; nothing is left anyway)
 #pragma unroll
-            for (int i = 0; i < NV * VEC; ++i) s += con_exp(val[i], m);
-        } else {
+        for (int i = 0; i < NV * VEC; ++i) s += con_exp(val[i], b);
+        s = sa_wave_sum_dpp(s);
+        PickPart p{sa_order(m), con_wave_min(top == m ? token : 0x7fffffff), m, s};
+        if (s != s) {  // a NaN: the first one is the largest value
+            token = 0x7fffffff;
 #pragma unroll
-            for (int i = 0; i < NV * VEC; ++i) s += val[i] == val[i] ? 0.0f : NAN;
+            for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+                for (int e = VEC - 1; e >= 0; --e)
+                    if (val[i * VEC + e] != val[i * VEC + e]) token = first + (i * NT + tid) * VEC + e;
+            p.best = sa_order(NAN);
+            p.token = con_wave_min(token);
         }
-        s = sa_block_sum<NT / 64>(s, scratch);
+        if (lane == 0) waves[tid >> 6] = p;
+        __syncthreads();
         if (tid == 0) {
-            for (int w = 0; w < NT / 64; ++w) key = best[w] > key ? best[w] : key;
-            if (nseg == 1) {
-                const bool none = (unsigned)(key >> 32) == sa_order(-INFINITY);
-                tokens[row] = none ? -1 : (long long)(unsigned)~(unsigned)key;
-                logp[row] = none ? -INFINITY : -logf(s);
-            } else {
-                part[blockIdx.x] = PickPart{key, m, s};
+            PickPart r = waves[0];
+#pragma unroll
+            for (int w = 1; w < NT / 64; ++w) {
+                pick_better(r, waves[w].best, waves[w].token);
+                r.m = fmaxf(r.m, waves[w].m);
             }
+            r.s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NT / 64; ++w)
+                if (waves[w].s != 0.0f) r.s += waves[w].s * con_exp(waves[w].m, r.m);
+            if (nseg == 1) pick_write(r, tokens + row, logp + row);
+            else part[blockIdx.x] = r;
         }
     }
 }
 
-// the segments of a row, in their order, by one wave
+// the segments of a row, by one wave
 __global__ __launch_bounds__(64) void pick_join_kernel(const PickPart* __restrict__ part, int nseg, long long* __restrict__ tokens,
                                                        float* __restrict__ logp) {
     const PickPart* P = part + (long)blockIdx.x * nseg;
-    unsigned long long key = 0;
-    float m = -INFINITY;
+    PickPart r{0u, 0x7fffffff, -INFINITY, 0.0f};
     for (int i = threadIdx.x; i < nseg; i += 64) {
-        key = P[i].key > key ? P[i].key : key;
-        m = fmaxf(m, P[i].m);
+        const PickPart p = P[i];
+        pick_better(r, p.best, p.token);
+        const float m = fmaxf(r.m, p.m);
+        r.s = (r.s != 0.0f ? r.s * con_exp(r.m, m) : 0.0f) + (p.s != 0.0f ? p.s * con_exp(p.m, m) : 0.0f);
+        r.m = m;
     }
+    const float m = sa_wave_max_dpp(r.m);
+    r.s = sa_wave_sum_dpp(r.s != 0.0f ? r.s * con_exp(r.m, m) : 0.0f);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const unsigned long long other = __shfl_xor(key, o, 64);
-        key = other > key ? other : key;
-    }
-    m = sa_wave_max(m);
-    float s = 0.f;
-    for (int i = threadIdx.x; i < nseg; i += 64)
-        if (P[i].m > -INFINITY || P[i].s != 0.0f) s += P[i].s * con_exp(P[i].m, m);
-    s = sa_wave_sum(s);
-    if (threadIdx.x == 0) {
-        const bool none = (unsigned)(key >> 32) == sa_order(-INFINITY);
-        tokens[blockIdx.x] = none ? -1 : (long long)(unsigned)~(unsigned)key;
-        logp[blockIdx.x] = none ? -INFINITY : -logf(s);
-    }
+    for (int o = 32; o > 0; o >>= 1) pick_better(r, (unsigned)__shfl_xor((int)r.best, o, 64), __shfl_xor(r.token, o, 64));
+    if (threadIdx.x == 0) pick_write(r, tokens + blockIdx.x, logp + blockIdx.x);
 }
 
-// Vectors a thread, segments a row, vectors a segment.  Segments as long as the registers and 48 KB of LDS allow -- each reads
-// the lists of its row again -- unless that leaves CUs without work; a row that one workgroup can hold is not split where that
-// would cost pick a second launch.
+// Vectors a thread, segments a row, vectors a segment.  Segments of 4096 tokens -- each reads the lists of its row again, and three
+// times as many of them run on a CU as of 8192 (256 x 131072 f32: 71 us; 8192 tokens 85, 2048 tokens 82) -- and shorter ones where
+// that leaves CUs without work.  Where it saves pick its second launch, one workgroup takes a row of up to 8192.
 struct ConPlan { int nv, nseg, per; };
 ConPlan con_plan(int rows, int V, int dtype, bool pick) {
-    const int vec = dtype == SA_F32 ? 4 : 8, most = dtype == SA_F32 ? 8 : 4, vectors = (V + 2 * vec - 2) / vec;
+    const int vec = dtype == SA_F32 ? 4 : 8, most = 16 / vec, vectors = (V + 2 * vec - 2) / vec;
     ConPlan p{1, 1, 0};
-    while (p.nv < most && 256 * p.nv < vectors &&
-           ((pick && vectors <= 256 * most) || (long)rows * ((vectors + 512 * p.nv - 1) / (512 * p.nv)) >= 512))
+    const bool whole = pick && vectors <= 512 * most;
+    while (256 * p.nv < vectors &&
+           (whole || (p.nv < most && (long)rows * ((vectors + 512 * p.nv - 1) / (512 * p.nv)) >= 512)))
         p.nv *= 2;
     p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
     p.per = (vectors + p.nseg - 1) / p.nseg;
@@ -245,7 +279,7 @@ void con_launch(const void* x, long ldx, void* y, long ldy, int rows, int V, con
     if (p.nv == 1) CON_LAUNCH(1);
     else if (p.nv == 2) CON_LAUNCH(2);
     else if (p.nv == 4) CON_LAUNCH(4);
-    else if constexpr (sizeof(T) == 4) CON_LAUNCH(8);
+    else if constexpr (PICK && sizeof(T) == 4) CON_LAUNCH(8);
 #undef CON_LAUNCH
 }
 
