@@ -280,30 +280,33 @@ class DistillFunction(torch.autograd.Function):
         _launch("sa_distill_loss", x, x.data_ptr(), None if dx is None else dx.data_ptr(), ld_outer, ld_inner, n_inner,
                 _DTYPES[x.dtype], rows, V, *args, None, 0, loss_rows.data_ptr(), loss.data_ptr())
         if dx is not None:
-            ctx.save_for_backward(x, values, ids, rest, targets, weights)
-            ctx.args = (ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale)
+            # (plain attributes and the version that save_for_backward would keep: six of its records cost more than the launches)
+            ctx.again = (x, x._version, values, ids, rest, targets, weights, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha,
+                         scale)
             ctx.dx = dx
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, go):
         from .ops import is_unit_gradient
-        none = (None,) * 8
+        if torch.is_grad_enabled():
+            raise SpeechAmdError("the distillation loss is differentiable once: its gradient is no function of the logits to autograd")
         # the first walk takes the buffer of the forward pass along: it is handed out once and never written again
         dx, ctx.dx = ctx.dx, None
         if dx is not None and is_unit_gradient(go):
-            return (dx,) + none
-        x, values, ids, rest, targets, weights = ctx.saved_tensors
-        ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale = ctx.args
+            return dx, None, None, None, None, None, None, None, None
+        (x, version, values, ids, rest, targets, weights, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha,
+         scale) = ctx.again
+        if x._version != version:
+            raise RuntimeError("the logits of the distillation loss were changed in place after its forward pass")
         fresh = dx is None
         if fresh:
             dx = torch.empty_like(x)
-        factor = go.detach().reshape(1).to(torch.float32)
+        factor = go.reshape(1).to(torch.float32)
         p = _lib.ptr
         _launch("sa_distill_loss", x, p(x), p(dx), ld_outer, ld_inner, n_inner, _DTYPES[x.dtype], rows, V, p(values), p(ids), p(rest), k,
                 p(targets), p(weights), temperature, alpha, scale, p(factor), 0 if fresh else 1, None, None)
-        return (dx,) + none
+        return dx, None, None, None, None, None, None, None, None
 
 
 class DistillLoss(torch.nn.Module):

@@ -503,6 +503,15 @@ def test_distill_factors_and_second_walks():
     assert torch.equal(leaf.grad, a.grad + b.grad)
     with torch.no_grad():
         assert not L().DistillLoss(2.0, 0.5)(leaf, **dev).requires_grad
+    # changed in place between the passes: a walk that needs the logits again says so; a second derivative is refused
+    from speech_amd._lib import SpeechAmdError
+    loss = L().DistillLoss(2.0, 0.5)(leaf, **dev)
+    with torch.no_grad():
+        leaf += 1
+    with pytest.raises(RuntimeError, match="in place"):
+        loss.backward()
+    with pytest.raises(SpeechAmdError, match="once"):
+        torch.autograd.grad(L().DistillLoss(2.0, 0.5)(leaf, **dev), leaf, create_graph=True)
 
 
 def test_distill_gradient_against_differences():
