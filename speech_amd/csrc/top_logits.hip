@@ -41,22 +41,48 @@ template <int LANES> __device__ __forceinline__ unsigned top_group(unsigned v) {
     return v;
 }
 
-// The largest prefix t (most significant bits first) that at least k of the 64 * N keys of this wave reach; stops where few
-// enough do.  Uniform over the wave.
-template <int N> __device__ __forceinline__ unsigned top_bound(const unsigned (&key)[N], int k) {
-    unsigned t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned u = t | (1u << bit);
+__device__ __forceinline__ unsigned top_wave_max(unsigned v) {  // row_shr 1, 2, 4, 8, row_bcast 15, 31
+#define TOP_DPP_MAX(ctrl, rows)                                                                          \
+    {                                                                                                    \
+        const unsigned o = (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, (ctrl), (rows), 0xf, false); \
+        v = o > v ? o : v;                                                                               \
+    }
+    TOP_DPP_MAX(0x111, 0xf) TOP_DPP_MAX(0x112, 0xf) TOP_DPP_MAX(0x114, 0xf) TOP_DPP_MAX(0x118, 0xf)
+    TOP_DPP_MAX(0x142, 0xa) TOP_DPP_MAX(0x143, 0xc)
+#undef TOP_DPP_MAX
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// A number that at least k of this wave's 64 * N keys reach, and few more than k: halving the stretch between the smallest and the
+// largest key until few enough do or the k-th key itself is found.  The low `shift` bits of the keys say nothing (logits of two
+// bytes) and are not searched.  Uniform over the wave.
+template <int N> __device__ __forceinline__ unsigned top_bound(unsigned (&key)[N], int k, int shift) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) key[i] >>= shift;
+    unsigned hi = key[0], lo = key[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        hi = key[i] > hi ? key[i] : hi;
+        lo = key[i] < lo ? key[i] : lo;
+    }
+    hi = top_wave_max(hi) + 1u;  // (no key is all ones: sa_order)
+    lo = ~top_wave_max(~lo);
+    while (hi - lo > 1) {  // at least k keys reach lo, fewer reach hi
+        const unsigned u = lo + (hi - lo) / 2;
         int c = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) c += __popcll(__ballot(key[i] >= u));
-        if (c >= k) {
-            t = u;
-            if (c <= k + (k >> 3)) break;
-        }
+        if (c < k) { hi = u; continue; }
+        lo = u;
+        if (c <= k + (k >> 3)) break;
     }
-    return t;
+    return lo << shift;
 }
+
+// the low bits of a key, which no logit of the type sets differently from its sign
+template <typename T> struct TopShift { static constexpr int value = 0; };
+template <> struct TopShift<SaBf16> { static constexpr int value = 16; };
+template <> struct TopShift<SaF16> { static constexpr int value = 13; };
 
 template <int NT> __device__ __forceinline__ int top_count(int c, int* scratch) {
 #pragma unroll
@@ -116,7 +142,8 @@ __device__ __forceinline__ void top_write_rest(float m, float s, float temperatu
 // A segment of a row: `per` <= NT * NV vectors; nseg == 1: the whole row, and the result.  (The segments of a row are of equal
 // length: a short last one would have fewer than k threads with anything, no bound, and take the exact way.)
 // It is a chain of short phases, and what hides one is another workgroup's: registers for six waves a SIMD (4096 x 32000 bf16, k = 64:
-// 88 us; for eight, with spills, 95; unbounded 132).
+// 85 - 90 us by box, where the bytes alone would take 52; registers for eight waves, with spills, 128; unbounded 132).  With the
+// exponentials left out it takes 75, without the ranking 76, with a bound known beforehand 58: no one phase bounds it.
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void top_segment_kernel(const T* __restrict__ x, SaRows at, int V, int k, int cap,
                                                          float temperature, int nseg, int per, TopOut out,
@@ -167,7 +194,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
         unsigned key[KEYS / 64];
 #pragma unroll
         for (int i = 0; i < KEYS / 64; ++i) key[i] = top[tid + 64 * i];
-        const unsigned t = top_bound(key, k);
+        const unsigned t = top_bound(key, k, TopShift<T>::value);
         if (tid == 0) bound = t;
     }
     __syncthreads();
@@ -186,18 +213,35 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
             const bool hit = f >= b;
             s += hit ? 0.0f : u;  // (NaN stays in the sum)
             hits[(i * VEC + e) / 32] = hits[(i * VEC + e) / 32] * 2u + (hit ? 1u : 0u);
+            if (e == VEC - 1) __builtin_amdgcn_sched_barrier(0);  // (one vector after the other)
         }
+    // Most threads that have one have one: their maximum.  The others' are read again (they were here a moment ago), two at a time.
+    unsigned long long left = 0;  // the first element in the highest bit
 #pragma unroll
-    for (int w = 0; w < WORDS; ++w)
-        while (hits[w]) {
-            const int j = w * 32 + BITS - 32 + __builtin_clz(hits[w]);
-            hits[w] &= ~(0x80000000u >> __builtin_clz(hits[w]));
-            const int v = first + (j / VEC * NT + tid) * VEC + j % VEC;
-            if (v >= 0 && v < end) {  // (read again: it was here a moment ago)
-                const int p = atomicAdd(&count, 1);
-                if (p < kCand) R.cand[p] = sa_rank_key(sa_widen(xr[v]), v);
+    for (int w = 0; w < WORDS; ++w) left |= (unsigned long long)hits[w] << (64 - BITS * (w + 1));
+    const int n = __popcll(left);
+    if (n) {
+        auto place = [&](int j) { return first + (j / VEC * NT + tid) * VEC + j % VEC; };
+        auto add = [&](int v, float f) {
+            if (v < 0 || v >= end) return;  // (what the row does not have was loaded as -inf)
+            const int p = atomicAdd(&count, 1);
+            if (p < kCand) R.cand[p] = sa_rank_key(f, v);
+        };
+        if (n == 1) {
+            add(place(__builtin_clzll(left)), mx);
+        } else {
+            while (left) {
+                const int j0 = __builtin_clzll(left), j1 = 63 - __builtin_ctzll(left), v0 = place(j0), v1 = place(j1);
+                const float f0 = v0 >= 0 && v0 < end ? sa_widen(xr[v0]) : 0.0f, f1 = v1 >= 0 && v1 < end ? sa_widen(xr[v1]) : 0.0f;
+                left &= ~(0x8000000000000000ull >> j0);
+                add(v0, f0);
+                if (j1 != j0) {
+                    left &= ~(0x8000000000000000ull >> j1);
+                    add(v1, f1);
+                }
             }
         }
+    }
     s = sa_block_sum<NT / 64>(s, sums);
     int C = count;
     float m = b;
@@ -252,7 +296,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
 // The segments of a row: the same over their candidates, nseg * cap <= NT * EACH keys, in registers.
 template <int NT, int EACH>
 __global__ __launch_bounds__(NT) void top_merge_kernel(const unsigned long long* __restrict__ lists, const TopPart* __restrict__ parts,
-                                                       int nseg, int cap, int k, float temperature, TopOut out) {
+                                                       int nseg, int cap, int k, int shift, float temperature, TopOut out) {
     __shared__ TopRank R;
     __shared__ unsigned top[256], bound;
     __shared__ int count, counts[NT / 64];
@@ -279,7 +323,7 @@ __global__ __launch_bounds__(NT) void top_merge_kernel(const unsigned long long*
         unsigned key[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) key[i] = top[tid + 64 * i];
-        const unsigned t = top_bound(key, k);
+        const unsigned t = top_bound(key, k, shift);
         if (tid == 0) bound = t;
     }
     __syncthreads();
@@ -388,8 +432,8 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x,
     if (lane == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
-// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88 us
-// whole, 90 + 23 in two segments and a merge); others are split into segments of 256 threads, shorter ones where there are few rows, as long as one workgroup can hold what the segments leave.
+// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88
+// us whole, 90 + 23 in two segments and a merge); others are split into segments of 256 threads, shorter ones where there are few rows, as long as one workgroup can hold what the segments leave.
 struct TopPlan {
     int nt, nv, nseg, per, cap;  // threads, vectors a thread, segments a row, vectors a segment, candidates a segment leaves
 };
@@ -445,7 +489,7 @@ void top_launch(const void* x, const SaRows& at, long rows, int V, int k, float 
     if (p.nseg == 1) return;
 #define TOP_MERGE(NT, EACH)                                                                                            \
     hipLaunchKernelGGL((top_merge_kernel<NT, EACH>), dim3((unsigned)rows), dim3(NT), 0, stream, (const unsigned long long*)lists, \
-                       (const TopPart*)parts, p.nseg, p.cap, k, temperature, out)
+                       (const TopPart*)parts, p.nseg, p.cap, k, TopShift<T>::value, temperature, out)
     if (n <= 256 * 8) TOP_MERGE(256, 8);
     else if (n <= 1024 * 8) TOP_MERGE(1024, 8);
     else TOP_MERGE(1024, 32);  // (129 segments of 224 at most: 28896 keys)
