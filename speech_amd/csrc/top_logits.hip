@@ -106,12 +106,12 @@ struct TopRank {
 };
 template <int NT>
 __device__ __forceinline__ unsigned long long top_rank(TopRank& R, int C, int k, long row, const TopOut& out) {
-    constexpr int PARTS = NT / 128;
-    const int tid = threadIdx.x, part = tid >> 7;
+    constexpr int WIDE = NT < 128 ? NT : 128, PARTS = NT / WIDE;
+    const int tid = threadIdx.x, part = tid / WIDE;
     for (int c = tid; c < kCand; c += NT) R.rank[c] = 0;
     const int each = (C + PARTS - 1) / PARTS, from = part * each, to = from + each < C ? from + each : C;
     __syncthreads();
-    for (int c = tid & 127; c < C; c += 128) {
+    for (int c = tid % WIDE; c < C; c += WIDE) {
         const unsigned long long key = R.cand[c];
         int rank = 0;
 #pragma unroll 4
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     constexpr int VEC = SaVec<T>::N;
     __shared__ TopRank R;
     // one key a thread, or, in rows so short that k threads might not have one, a key an element
-    constexpr int KEYS = NV == 1 ? NT * VEC : 256;
+    constexpr int KEYS = NT == 64 ? 64 : NV == 1 ? NT * VEC : 256;
     __shared__ unsigned top[KEYS], bound;
     __shared__ int count, counts[NT / 64];
     __shared__ float sums[NT / 64];
@@ -166,36 +166,52 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, first + (i * NT + tid) * VEC, end);
     const int lo = first < 0 ? 0 : first, valid = end > lo ? end - lo : 0;
 
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, sa_element<T>(raw[i], e));
     // (two-byte logits are widened again for every use: kept as 32 bits over the barriers they would take twice the registers)
     auto again = [&] {
         if constexpr (sizeof(T) == 2)
 #pragma unroll
             for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
     };
-    again();
-    if constexpr (NV == 1) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float f = sa_element<T>(raw[0], e);
-            top[e * NT + tid] = f == f ? sa_order(f) : 0u;
-        }
-    } else {
-        const unsigned u = top_group<NT / 256>(sa_order(mx));
-        if (tid % (NT / 256) == 0) top[tid / (NT / 256)] = u;
-    }
+    float mx = -INFINITY;
     if (tid == 0) count = 0;
-    __syncthreads();
-    if (tid < 64) {
-        unsigned key[KEYS / 64];
+    if constexpr (NT == 64) {  // one wave: eight keys a lane, and no exchange
+        constexpr int GROUP = NV * VEC / 8;
+        unsigned key[8];
 #pragma unroll
-        for (int i = 0; i < KEYS / 64; ++i) key[i] = top[tid + 64 * i];
+        for (int g = 0; g < 8; ++g) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = g * GROUP; j < (g + 1) * GROUP; ++j) m = fmaxf(m, sa_element<T>(raw[j / VEC], j % VEC));
+            key[g] = sa_order(m);
+            mx = fmaxf(mx, m);
+        }
+        again();
         const unsigned t = top_bound(key, k, TopShift<T>::value);
         if (tid == 0) bound = t;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, sa_element<T>(raw[i], e));
+        again();
+        if constexpr (NV == 1) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float f = sa_element<T>(raw[0], e);
+                top[e * NT + tid] = f == f ? sa_order(f) : 0u;
+            }
+        } else {
+            const unsigned u = top_group<(NT < 256 ? 256 : NT) / 256>(sa_order(mx));
+            if (tid % ((NT + 255) / 256) == 0) top[tid / ((NT + 255) / 256)] = u;
+        }
+        __syncthreads();
+        if (tid < 64) {
+            unsigned key[KEYS / 64];
+#pragma unroll
+            for (int i = 0; i < KEYS / 64; ++i) key[i] = top[tid + 64 * i];
+            const unsigned t = top_bound(key, k, TopShift<T>::value);
+            if (tid == 0) bound = t;
+        }
     }
     __syncthreads();
     const float b = bound <= sa_order(-INFINITY) ? -INFINITY : sa_unorder(bound);
@@ -286,7 +302,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     top_rank<NT>(R, C, k, row, out);
     // the candidates that were not taken belong to the others
     const float mu = C > k ? R.others[0] : -INFINITY;
-    const float su = sa_block_sum<NT / 64>(tid < C - k ? top_exp(R.others[tid], mu, c) : 0.0f, sums);
+    float su = 0.0f;
+    for (int i = tid; i < C - k; i += NT) su += top_exp(R.others[i], mu, c);
+    su = sa_block_sum<NT / 64>(su, sums);
     if (tid == 0) {
         const float M = fmaxf(m, mu);
         top_write_rest(M, s * top_exp(m, M, c) + su * top_exp(mu, M, c), temperature, out.rest + row);
@@ -432,15 +450,21 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x,
     if (lane == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
-// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88
-// us whole, 90 + 23 in two segments and a merge); others are split into segments of 256 threads, shorter ones where there are few rows, as long as one workgroup can hold what the segments leave.
+// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88 us
+// whole, 90 + 23 in two segments and a merge), and a wave takes a row of up to 1000 (2000 of two bytes) when every SIMD gets one:
+// no exchange between waves (16000 x 1000 f32, k = 8: 25 us against 58 with 256 threads; 16000 x 1000 bf16, k = 64: 40 against 98; at twice
+// the length 33 against 36 and 32 against 30).  Others are split into segments of 256 threads, shorter ones where there are few
+// rows, as long as one workgroup can hold what the segments leave.
 struct TopPlan {
     int nt, nv, nseg, per, cap;  // threads, vectors a thread, segments a row, vectors a segment, candidates a segment leaves
 };
 TopPlan top_plan(long rows, int V, int k, int dtype) {
     const int vec = dtype == SA_F32 ? 4 : 8, vectors = (V + vec - 1 + vec - 1) / vec;  // the longest row, with its lead
     TopPlan p{256, 8, 1, vectors, k + k / 2 + 32};
-    if (vectors <= 256 * 8) {
+    if (vectors <= 64 * 4 && rows >= 1024) {
+        p.nt = 64;
+        p.nv = vectors <= 128 ? 2 : 4;
+    } else if (vectors <= 256 * 8) {
         p.nv = vectors <= 256 ? 1 : vectors <= 512 ? 2 : vectors <= 1024 ? 4 : 8;
     } else if (vectors <= 1024 * 8 && rows >= 256) {
         p.nt = vectors <= 512 * 8 ? 512 : 1024;
@@ -479,7 +503,9 @@ void top_launch(const void* x, const SaRows& at, long rows, int V, int k, float 
 #define TOP_LAUNCH(NT, NV)                                                                                                   \
     hipLaunchKernelGGL((top_segment_kernel<T, NT, NV>), grid, block, 0, stream, xt, at, V, k, cap, temperature, p.nseg, p.per, out, \
                        lists, parts)
-    if (p.nt == 1024) TOP_LAUNCH(1024, 8);
+    if (p.nt == 64 && p.nv == 2) TOP_LAUNCH(64, 2);
+    else if (p.nt == 64) TOP_LAUNCH(64, 4);
+    else if (p.nt == 1024) TOP_LAUNCH(1024, 8);
     else if (p.nt == 512) TOP_LAUNCH(512, 8);
     else if (p.nv == 1) TOP_LAUNCH(256, 1);
     else if (p.nv == 2) TOP_LAUNCH(256, 2);

@@ -68,7 +68,8 @@ def constraints(g, n, V, length, biases, grammar, scalars=False):
 SHAPES = [(1, 1, 0, 0, True), (2, 29, 40, 3, True), (32, 29, 200, 0, True), (3, 32, 7, 50, False), (5, 1000, None, 9, True),
           (3, 4095, 300, 20, True), (2, 4096, 5000, 0, False), (4, 4097, 64, 64, True), (3, 8193, 600, 10, True), (2, 16385, 1, 1, True),
           (2, 32000, 1500, 128, True), (7, 50021, 333, 16, True), (2, 131072, 4096, 100, True), (1, 262147, 70, 5, False),
-          (1, 1048576, 900, 300, True), (1, 1044481, 64, 0, False), (130, 8190, 20, 2, True)]
+          (1, 1048576, 900, 300, True), (1, 1044481, 64, 0, False), (130, 8190, 20, 2, True),
+          (600, 8190, 9, 3, True)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -208,14 +209,17 @@ def check_top(x, k, temperature=1.0, got=None):
 @pytest.mark.parametrize("n,V,k", [(1, 1, 1), (5, 2, 2), (40, 29, 8), (700, 29, 29), (9, 64, 5), (9, 65, 33), (6, 128, 128), (3, 129, 128),
                                    (4, 511, 20), (4, 1000, 64), (3, 4099, 100), (2, 8192, 1), (2, 8195, 128), (3, 32000, 64),
                                    (2, 50021, 100), (3, 131071, 128), (1, 300007, 50),
-                                   (1, 1048576, 128), (1, 1044483, 20)])
+                                   (1, 1048576, 128), (1, 1044483, 20),
+                                   # enough rows for a wave each, for a workgroup each, and just too few
+                                   (1100, 131, 5), (1024, 257, 128), (1030, 1000, 64), (1100, 1021, 100), (1023, 1000, 64), (1040, 2003, 33),
+                                   (260, 8200, 20), (256, 20000, 64), (255, 20000, 64), (257, 32768, 128), (258, 33001, 7)])
 def test_top_logits(n, V, k, dtype):
     check_top(rows_like(gen(V + k), n, V, dtype), k, 1.0 if n % 2 else 2.5)
 
 
-@pytest.mark.parametrize("V", [29, 300, 5000, 40000])
+@pytest.mark.parametrize("V,times", [(29, 1), (300, 1), (5000, 1), (40000, 1), (300, 74), (1000, 74), (9000, 19), (30000, 19)])
 @pytest.mark.parametrize("k", [1, 20, 128])
-def test_top_logits_of_rows_that_are_not_ordinary(V, k):
+def test_top_logits_of_rows_that_are_not_ordinary(V, times, k):
     k = min(k, V)
     g = gen(V * k)
     x = torch.randn(14, V, generator=g)
@@ -235,7 +239,15 @@ def test_top_logits_of_rows_that_are_not_ordinary(V, k):
     x[13] = -x[13].abs() - 100
     for dtype in TYPES:
         y = x.to(dtype)
-        check_top(y, k, 1.0)
+        if times == 1:
+            check_top(y, k, 1.0)
+            continue
+        many = L().top_logits(y.cuda().repeat(times, 1), k)   # other launch shapes; every copy of a row has the same answer
+        many = [t.view(times, 14, *t.shape[1:]) for t in many]
+        for t in many:
+            bits = t.view(torch.int32) if t.dtype == torch.float32 else t
+            assert bool((bits == bits[:1]).all())
+        check_top(y, k, 1.0, got=[t[0] for t in many])
 
 
 @pytest.mark.parametrize("V", [9001, 40000, 200001])
