@@ -142,12 +142,12 @@ __device__ __forceinline__ void top_write_rest(float m, float s, float temperatu
 // A segment of a row: `per` <= NT * NV vectors; nseg == 1: the whole row, and the result.  (The segments of a row are of equal
 // length: a short last one would have fewer than k threads with anything, no bound, and take the exact way.)
 // It is a chain of short phases, and what hides one is another workgroup's: registers for six waves a SIMD (4096 x 32000 bf16, k = 64:
-// 85 - 90 us by box, where the bytes alone would take 52; registers for eight waves, with spills, 128; unbounded 132).  With the
-// exponentials left out it takes 75, without the ranking 76, with a bound known beforehand 58: no one phase bounds it.
+// 81 us on most boxes, where the bytes alone would take 52; registers for eight waves, with spills, 128; unbounded 132).  Without the
+// exponentials it takes 75, without the ranking 76, with a bound known beforehand 58: no one phase bounds it.
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void top_segment_kernel(const T* __restrict__ x, SaRows at, int V, int k, int cap,
-                                                         float temperature, int nseg, int per, TopOut out,
-                                                         unsigned long long* __restrict__ lists, TopPart* __restrict__ parts) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void top_segment_kernel(
+    const T* __restrict__ x, SaRows at, int V, int k, int cap, float temperature, int nseg, int per, TopOut out,
+    unsigned long long* __restrict__ lists, TopPart* __restrict__ parts) {
     constexpr int VEC = SaVec<T>::N;
     __shared__ TopRank R;
     // one key a thread, or, in rows so short that k threads might not have one, a key an element
@@ -166,14 +166,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, first + (i * NT + tid) * VEC, end);
     const int lo = first < 0 ? 0 : first, valid = end > lo ? end - lo : 0;
 
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, sa_element<T>(raw[i], e));
     // (two-byte logits are widened again for every use: kept as 32 bits over the barriers they would take twice the registers)
     auto again = [&] {
         if constexpr (sizeof(T) == 2)
 #pragma unroll
             for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
     };
-    float mx = -INFINITY;
-    if (tid == 0) count = 0;
+    again();
     if constexpr (NT == 64) {  // one wave: eight keys a lane, and no exchange
         constexpr int GROUP = NV * VEC / 8;
         unsigned key[8];
@@ -183,17 +187,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
 #pragma unroll
             for (int j = g * GROUP; j < (g + 1) * GROUP; ++j) m = fmaxf(m, sa_element<T>(raw[j / VEC], j % VEC));
             key[g] = sa_order(m);
-            mx = fmaxf(mx, m);
         }
-        again();
         const unsigned t = top_bound(key, k, TopShift<T>::value);
-        if (tid == 0) bound = t;
+        if (tid == 0) { bound = t; count = 0; }
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, sa_element<T>(raw[i], e));
-        again();
         if constexpr (NV == 1) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -204,6 +201,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
             const unsigned u = top_group<(NT < 256 ? 256 : NT) / 256>(sa_order(mx));
             if (tid % ((NT + 255) / 256) == 0) top[tid / ((NT + 255) / 256)] = u;
         }
+        if (tid == 0) count = 0;
         __syncthreads();
         if (tid < 64) {
             unsigned key[KEYS / 64];
@@ -229,7 +227,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
             const bool hit = f >= b;
             s += hit ? 0.0f : u;  // (NaN stays in the sum)
             hits[(i * VEC + e) / 32] = hits[(i * VEC + e) / 32] * 2u + (hit ? 1u : 0u);
-            if (e == VEC - 1) __builtin_amdgcn_sched_barrier(0);  // (one vector after the other)
+            if (e == VEC - 1) __builtin_amdgcn_sched_barrier(0);  // (one vector after the other: fewer registers, 85 -> 81 us)
         }
     // Most threads that have one have one: their maximum.  The others' are read again (they were here a moment ago), two at a time.
     unsigned long long left = 0;  // the first element in the highest bit
@@ -302,8 +300,9 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     top_rank<NT>(R, C, k, row, out);
     // the candidates that were not taken belong to the others
     const float mu = C > k ? R.others[0] : -INFINITY;
-    float su = 0.0f;
-    for (int i = tid; i < C - k; i += NT) su += top_exp(R.others[i], mu, c);
+    float su = tid < C - k ? top_exp(R.others[tid], mu, c) : 0.0f;
+    if constexpr (NT < kCand)
+        for (int i = tid + NT; i < C - k; i += NT) su += top_exp(R.others[i], mu, c);
     su = sa_block_sum<NT / 64>(su, sums);
     if (tid == 0) {
         const float M = fmaxf(m, mu);
@@ -450,7 +449,7 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x,
     if (lane == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
-// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 88 us
+// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 81 us
 // whole, 90 + 23 in two segments and a merge), and a wave takes a row of up to 1000 (2000 of two bytes) when every SIMD gets one:
 // no exchange between waves (16000 x 1000 f32, k = 8: 25 us against 58 with 256 threads; 16000 x 1000 bf16, k = 64: 40 against 98; at twice
 // the length 33 against 36 and 32 against 30).  Others are split into segments of 256 threads, shorter ones where there are few
