@@ -615,7 +615,7 @@ ctcStatus_t sa_s2s_greedy_decode_constrained(const float* eh, const float* const
 
 /* The k largest logits of every row (k <= V, k <= SA_TOP_MAX) in descending order, ties to the lowest index, NaN above
  * everything: values (rows, k) float, ids (rows, k) int64, and rest[row] = log sum exp(x_v / temperature) over the OTHER V - k
- * tokens (-inf when there are none) -- what a distillation loss needs of a teacher's row.
+ * tokens (-inf when there are none) -- what a distillation loss needs of a teacher's row.  1e-6 <= temperature <= 1e6.
  * Row r starts at x + (r / n_inner) * ld_outer + (r % n_inner) * ld_inner. */
 size_t sa_top_logits_workspace_bytes(long rows, int V, int k, int dtype);
 ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner, int n_inner, int dtype, long rows, int V, int k,

@@ -409,7 +409,7 @@ extern "C" ctcStatus_t sa_distill_loss(const void* x, void* dx, long ld_outer, l
                                        void* stream_) {
     SA_CLEAR_ERR();
     if (rows < 0 || rows > 0x7fffffffL || n_inner < 1 || !sa_rows_ok(dtype, V) || k < 1 || k > SA_TOP_MAX ||
-        !(temperature > 0.f) || !(temperature < INFINITY) || !(alpha >= 0.f && alpha <= 1.f) || (rows > 0 && !loss && !dx) ||
+        !sa_temperature_ok(temperature) || !(alpha >= 0.f && alpha <= 1.f) || (rows > 0 && !loss && !dx) ||
         (loss && !loss_rows && rows > 0))
         return CTC_STATUS_INVALID_VALUE;
     hipStream_t stream = (hipStream_t)stream_;

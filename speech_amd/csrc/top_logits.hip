@@ -328,7 +328,7 @@ __global__ __launch_bounds__(NT) void top_merge_kernel(const unsigned long long*
     unsigned long long keys[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) keys[i] = i * NT + tid < n ? lists[i * NT + tid] : 0;
-    const TopPart P = tid < nseg ? parts[tid] : TopPart{-INFINITY, 0.0f};  // (nseg <= 256)
+    const TopPart P = tid < nseg ? parts[tid] : TopPart{-INFINITY, 0.0f};  // (nseg <= 62 here with 256 threads, <= 257 with 1024)
     unsigned long long mx = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) mx = keys[i] > mx ? keys[i] : mx;
@@ -536,7 +536,7 @@ extern "C" ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner
                                      int k, float temperature, float* values, long long* ids, float* rest, void* workspace,
                                      size_t workspace_bytes, void* stream) {
     SA_CLEAR_ERR();
-    if (!top_ok(rows, V, k, dtype) || n_inner < 1 || !(temperature > 0.f) || !(temperature < INFINITY))
+    if (!top_ok(rows, V, k, dtype) || n_inner < 1 || !sa_temperature_ok(temperature))
         return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
     const TopPlan p = top_plan(rows, V, k, dtype);

@@ -176,7 +176,7 @@ def decoding_constraints(rows, V, dev, repetition=None, presence=None, frequency
 
 def _matrix(logits):
     ld, _, _, rows = _rows_of(logits)
-    if logits.dim() != 2:
+    if logits.dim() != 2 or rows > 0x7fffffff:
         raise SpeechAmdError("logits must be (requests, V), got %s" % (tuple(logits.shape),))
     return ld, rows, logits.shape[1]
 
@@ -206,6 +206,7 @@ def constrain(logits, history=None, lengths=None, repetition=None, presence=None
             raise SpeechAmdError("constrain writes to out without recording it: out must not require a gradient")
     _launch("sa_logits_constrain", logits, logits.data_ptr(), ld, _DTYPES[logits.dtype], out.data_ptr(), out.stride(0), rows, V,
             ctypes.byref(c))
+    torch.autograd.graph.increment_version(out)  # (written behind autograd's back: whoever saved it must see that)
     return out
 
 
@@ -230,15 +231,16 @@ def pick(logits, history=None, lengths=None, repetition=None, presence=None, fre
 
 def _temperature(t):
     t = float(t)
-    if not (t > 0.0 and math.isfinite(t)):
-        raise SpeechAmdError("temperature must be positive and finite, got %r" % t)
+    if not 1e-6 <= t <= 1e6:  # (beyond it T^2 or logits / T leave float32)
+        raise SpeechAmdError("temperature must be within 1e-6 .. 1e6, got %r" % t)
     return t
 
 
 def top_logits(logits, k, temperature=1.0):
     """The k largest logits of every row of (..., V): (values (..., k) float32, ids (..., k) int64, rest (...) float32).
     Descending; ties go to the lowest id; NaN counts as the largest value.  rest = log sum exp(logits / temperature) over the
-    other V - k classes (-inf when there are none): with it DistillLoss knows how much of the teacher the list leaves out."""
+    other V - k classes (-inf when there are none): with it DistillLoss knows how much of the teacher the list leaves out.
+    Not differentiable."""
     ld_outer, ld_inner, n_inner, rows = _rows_of(logits)
     V, k, t = logits.shape[-1], int(k), _temperature(temperature)
     if not 1 <= k <= min(V, TOP_MAX):
@@ -320,15 +322,16 @@ class DistillLoss(torch.nn.Module):
 
     forward(logits (..., V), values (..., k) float32, ids (..., k) int64, rest=None (...) float32, targets=None (...) int64,
     weights=None (...) float32) -> (1,) float32.  An id that is no class is absent from the list (padding), a target that is none
-    gives no hard term, a row of weight 0 is not read and has a gradient of 0 whatever it holds."""
+    gives no hard term, a row of weight 0 is not read and has a gradient of 0 whatever it holds.  Only the logits get a gradient,
+    in their own type; it is differentiable once."""
 
     def __init__(self, temperature=1.0, alpha=1.0, denom=None):
         super().__init__()
         self.temperature, self.alpha, self.denom = _temperature(temperature), float(alpha), denom
         if not 0.0 <= self.alpha <= 1.0:
             raise SpeechAmdError("alpha must be within 0 .. 1, got %r" % alpha)
-        if denom is not None and not (float(denom) > 0.0 and math.isfinite(float(denom))):
-            raise SpeechAmdError("denom must be positive and finite, got %r" % denom)
+        if denom is not None and not 1e-30 <= float(denom) <= 1e30:
+            raise SpeechAmdError("denom must be within 1e-30 .. 1e30, got %r" % denom)
 
     def forward(self, logits, values, ids, rest=None, targets=None, weights=None):
         if not torch.is_tensor(values) or not 1 <= values.shape[-1] <= TOP_MAX:

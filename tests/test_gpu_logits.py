@@ -176,6 +176,23 @@ def test_constrain_in_place_on_rows_with_gaps(V, ld, off, dtype):
     assert float((la - lb).abs().max()) <= 2 * ((3 * 60 + 42) * U + 2 * U * float(la.abs().max()))
 
 
+def test_lists_and_masks_that_are_views():
+    """Histories, bias lists and masks as stretches of wider tensors (a token matrix that is still being written, ...)."""
+    g = gen(33)
+    n, V = 6, 5003
+    x = rows_like(g, n, V, torch.float32)
+    kw = constraints(g, n, V, 60, 9, True)
+    want = ref.constrain(x, **kw)
+    wide = dict(kw)
+    for name, pad in (("history", 11), ("bias_ids", 4), ("bias_values", 4), ("mask", 3)):
+        t = torch.randint(0, 9, (kw[name].shape[0], kw[name].shape[1] + 2 * pad), generator=g).to(kw[name].dtype)
+        t[:, pad:-pad] = kw[name]
+        wide[name] = t.cuda()[:, pad:-pad]
+    got = L().constrain(x.cuda(), **cuda(wide))
+    assert torch.equal(got, L().constrain(x.cuda(), **cuda(kw)))
+    assert torch.equal(L().pick(x.cuda(), **cuda(wide))[0].cpu(), ref.pick(want)[0])
+
+
 def test_constrain_refuses_on_the_gpu():
     from speech_amd._lib import SpeechAmdError
     x = torch.zeros(3, 40).cuda()
@@ -186,6 +203,9 @@ def test_constrain_refuses_on_the_gpu():
             L().constrain(x, **kw)
     with pytest.raises(SpeechAmdError):
         L().pick(torch.zeros(2, 3, 40).cuda())
+    seen = x._version   # written in place: whoever saved the tensor must see that
+    L().constrain(x, out=x)
+    assert x._version > seen
     assert L().constrain(x[:0]).shape == (0, 40) and L().pick(x[:0])[0].shape == (0,)
 
 
@@ -388,7 +408,8 @@ DSHAPES = [(1, 1, 1), (3, 2, 1), (40, 29, 8), (7, 29, 29), (6, 64, 10), (5, 130,
 def test_distill(n, V, k, dtype):
     g = gen(V + k)
     denom = n / 256.0 if dtype == torch.float16 else None     # small gradients vanish in float16 without a loss scale
-    for rest, alpha, temperature in ((True, 0.7, 2.0), (False, 1.0, 1.0), (True, 1.0, 1.0), (False, 0.4, 4.0)):
+    for rest, alpha, temperature in ((True, 0.7, 2.0), (False, 1.0, 1.0), (True, 1.0, 1.0), (False, 0.4, 4.0),
+                                     (True, 0.5, 3.0), (False, 0.3, 0.7), (True, 1.0, 5.0), (True, 0.0, 2.0), (False, 0.5, 1.0)):
         x, kw = student(g, n, V, dtype, k, temperature, rest, alpha < 1, n % 2 == 1)
         check_distill(x, kw, temperature, alpha, denom)
 
@@ -424,6 +445,8 @@ def test_distill_of_rows_that_are_not_ordinary(V):
     pick = lambda d, at: {a: (b[at] if torch.is_tensor(b) else b) for a, b in d.items()}  # noqa: E731
     check_distill(x[keep], pick(kw, keep), 2.0, 0.6)
     check_distill(x[keep], dict(pick(kw, keep), rest=None), 2.0, 0.6)
+    for temperature in (1.0, 3.0, 4.0):   # (the lists are numbers like any others at these temperatures)
+        check_distill(x[keep], pick(kw, keep), temperature, 0.6)
     # the row of lowest values by itself: its spread is the type's, the bound above would say nothing
     leaf = x[10:11].cuda().requires_grad_(True)
     one = cuda(pick(kw, [10]))

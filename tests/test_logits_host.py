@@ -84,7 +84,7 @@ def test_parameters_of_the_loss_are_checked():
         L.DistillLoss(alpha=0.5)(x, v, i)
     with pytest.raises(SpeechAmdError, match="k"):
         L.DistillLoss()(x, torch.zeros(2, 129), torch.zeros(2, 129, dtype=torch.int64))
-    for t in (0.0, -1.0, math.nan, math.inf):
+    for t in (0.0, -1.0, math.nan, math.inf, 1e-9, 1e9):
         with pytest.raises(SpeechAmdError, match="temperature"):
             L._temperature(t)
 
@@ -125,7 +125,25 @@ def test_the_c_entries_refuse_before_they_launch():
         return lib.sa_distill_loss(x, dx, V, 0, 1, 0, rows, V, P, P, None, k, None, None, t, alpha, 1.0, None, 0, loss_rows,
                                    loss, None)
     assert dis(k=0) == dis(k=129) == dis(t=0.0) == dis(t=math.nan) == dis(alpha=1.5) == dis(alpha=math.nan) == bad
+    assert top(t=1e-9) == top(t=1e9) == dis(t=1e-9) == dis(t=1e9) == bad
     assert dis(x=None) == dis(rows=-1) == dis(loss_rows=None) == dis(loss=None, dx=None) == dis(V=0) == bad
+
+
+def test_the_constrained_decode_refuses_before_it_launches():
+    lib = _lib.lib()
+    P, bad = 1 << 12, 2
+    plist = (ctypes.c_void_p * 11)(*[P] * 11)
+    c = _lib.saConstraints()
+    c.repetition_all = 1.0
+
+    def run(con=c, end=3, max_len=4, states=None, following=None, ws=1 << 30, B=2, K=13):
+        return lib.sa_s2s_greedy_decode_constrained(P, plist, B, 20, 16, 16, 15, K, 1.0, end, max_len, 8,
+                                                    None if con is None else ctypes.byref(con), 1, states, following, P, P, P, ws,
+                                                    None)
+    assert run(con=None) == run(end=-1) == run(end=13) == run(max_len=0) == run(max_len=L.LIST_MAX) == bad
+    assert run(following=P) == run(ws=16) == run(B=0) == bad
+    c.mask, c.n_states, c.mask_ld = P, 2, 1
+    assert run(states=None) == bad
 
 
 def test_pack_mask():
