@@ -555,7 +555,8 @@ ctcStatus_t sa_argmax_rows(const float* x, long long* out, long rows, int K, voi
 /* ------------------------------------------------------------------------------------------------------------------
  * 9. Output rows: a row is the V logits of one token (a CTC frame, a decoder step).  Logits are SA_F32, SA_BF16 or SA_F16 with
  *    a last stride of one; every sum, maximum and penalty is held in 32 bits and a result is rounded to the logits' type once.
- *    Nothing here waits for the stream or keeps state; results do not depend on timing (integer atomics only).
+ *    Nothing here waits for the stream or keeps state; results do not depend on timing (integer atomics only).  A
+ *    launch has 32 (short rows) to 1024 threads a row, or 256 for each 2048 to 16384 bytes of it: what needs 2^32 is refused.
  *
  *    Constraints on the next token of a batch of requests, applied in this order to row b, token v, where c is how often v stands
  *    in the first lengths[b] entries of history row b (entries outside [0, V) count nowhere):
@@ -630,7 +631,7 @@ ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner, int n_inn
  *     hard = log sum exp(x) - x[target]                                    (0 for a target outside [0, V), or targets NULL)
  *     loss_rows[i] = scale * weights[i] * (alpha * temperature^2 * soft + (1 - alpha) * hard);   *loss = their sum
  * A row of weight 0 is not read: its loss and its gradient are 0 whatever it holds.  weights NULL: 1.
- * dx (the layout of x, or NULL) = the gradient of *loss with respect to x, times *d_factor when d_factor != NULL.
+ * dx (the layout of x, no part of it shared with x, or NULL) = the gradient of *loss with respect to x, times *d_factor when d_factor != NULL.
  * loss == NULL: only the gradient; then skip_unit != 0 leaves dx untouched when *d_factor is 1 (dx holds it already).
  * loss_rows (rows floats) is written whenever loss is. */
 ctcStatus_t sa_distill_loss(const void* x, void* dx, long ld_outer, long ld_inner, int n_inner, int dtype, long rows,

@@ -387,6 +387,9 @@ bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const
 // keeps what it can in LDS: 1024 threads, 256 KB in registers and 128 KB in LDS (2048 x 131072 f32: 440 us; without LDS 534, two
 // smaller workgroups on a CU 580 - 615, all of them bound by what is read twice).  A short row is one wave's, without any exchange
 // (16000 x 1000 f32: 31 us against 54 with 256 threads, 8000 x 2000 bf16: 24.5 against 41.6).
+int dis_threads(int vectors, int vec) {
+    return vectors <= 64 * 4 ? 64 : vectors <= 256 * 4 ? 256 : vectors <= 512 * 64 / vec ? 512 : 1024;
+}
 template <typename T>
 bool dis_launch(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
     constexpr int VEC = SaVec<T>::N;
@@ -412,6 +415,8 @@ extern "C" ctcStatus_t sa_distill_loss(const void* x, void* dx, long ld_outer, l
         !sa_temperature_ok(temperature) || !(alpha >= 0.f && alpha <= 1.f) || (rows > 0 && !loss && !dx) ||
         (loss && !loss_rows && rows > 0))
         return CTC_STATUS_INVALID_VALUE;
+    const int vec = dtype == SA_F32 ? 4 : 8;
+    if (!sa_threads_ok(rows, dis_threads((V + 2 * vec - 2) / vec, vec))) return CTC_STATUS_INVALID_VALUE;
     hipStream_t stream = (hipStream_t)stream_;
     if (rows > 0) {
         if (!x || !values || !ids) return CTC_STATUS_INVALID_VALUE;

@@ -204,9 +204,9 @@ def constrain(logits, history=None, lengths=None, repetition=None, presence=None
             raise SpeechAmdError("out must be like the logits, without overlapping rows")
         if out.requires_grad and torch.is_grad_enabled():
             raise SpeechAmdError("constrain writes to out without recording it: out must not require a gradient")
+    torch.autograd.graph.increment_version(out)  # (written behind autograd's back: whoever saved it must see that)
     _launch("sa_logits_constrain", logits, logits.data_ptr(), ld, _DTYPES[logits.dtype], out.data_ptr(), out.stride(0), rows, V,
             ctypes.byref(c))
-    torch.autograd.graph.increment_version(out)  # (written behind autograd's back: whoever saved it must see that)
     return out
 
 
@@ -257,6 +257,11 @@ def top_logits(logits, k, temperature=1.0):
     return values, ids, rest
 
 
+def _versions(tensors):
+    """How often each has been written to (a tensor made in inference mode does not count that)."""
+    return [None if t is None or t.is_inference() else t._version for t in tensors]
+
+
 class DistillFunction(torch.autograd.Function):
     """The summed loss (1,) of DistillLoss.  The gradient is produced in the forward pass; autograd's factor is applied by the
     kernel, in 32 bits and before the one rounding to the logits' type."""
@@ -282,9 +287,11 @@ class DistillFunction(torch.autograd.Function):
         _launch("sa_distill_loss", x, x.data_ptr(), None if dx is None else dx.data_ptr(), ld_outer, ld_inner, n_inner,
                 _DTYPES[x.dtype], rows, V, *args, None, 0, loss_rows.data_ptr(), loss.data_ptr())
         if dx is not None:
-            # (plain attributes and the version that save_for_backward would keep: six of its records cost more than the launches)
-            ctx.again = (x, x._version, values, ids, rest, targets, weights, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha,
-                         scale)
+            # (the logits are freed by the walk; the lists are plain attributes with the versions that save_for_backward would keep:
+            # six of its records cost more than the launches)
+            ctx.save_for_backward(x)
+            lists = (values, ids, rest, targets, weights)
+            ctx.again = (lists, _versions(lists), ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale)
             ctx.dx = dx
         return loss
 
@@ -297,10 +304,11 @@ class DistillFunction(torch.autograd.Function):
         dx, ctx.dx = ctx.dx, None
         if dx is not None and is_unit_gradient(go):
             return dx, None, None, None, None, None, None, None, None
-        (x, version, values, ids, rest, targets, weights, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha,
-         scale) = ctx.again
-        if x._version != version:
-            raise RuntimeError("the logits of the distillation loss were changed in place after its forward pass")
+        x, = ctx.saved_tensors
+        lists, versions, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale = ctx.again
+        if _versions(lists) != versions:
+            raise RuntimeError("the teacher's list, targets or weights of a distillation loss were changed in place after its forward pass")
+        values, ids, rest, targets, weights = lists
         fresh = dx is None
         if fresh:
             dx = torch.empty_like(x)

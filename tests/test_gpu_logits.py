@@ -270,6 +270,35 @@ def test_top_logits_of_rows_that_are_not_ordinary(V, times, k):
         check_top(y, k, 1.0, got=[t[0] for t in many])
 
 
+@pytest.mark.parametrize("V,times", [(129, 1), (700, 1), (1000, 64), (9000, 16), (30000, 16), (40000, 1), (200001, 1)])
+@pytest.mark.parametrize("k", [5, 128])
+def test_top_logits_of_masked_rows(V, times, k):
+    """A mask that leaves fewer than k, exactly k, a few more or many more, at both ends and between; NaN in many places."""
+    g = gen(V + k)
+    kept = [0, 1, k - 1, k, k + 1, k + 40, 2 * k + 200]
+    rows = []
+    for fill in (-math.inf, -60000.0, 0.0):
+        for n in kept:
+            x = torch.full((V,), fill)
+            at = torch.randperm(V, generator=g)[:n] if n % 2 else torch.arange(V)[-n:] if n else torch.arange(0)
+            x[at] = torch.randn(len(at), generator=g) * 3 + (5 if fill == 0.0 else 0)
+            rows.append(x)
+    for n in (k // 2 + 1, min(V, 300), min(V, 2 * k + 300)):
+        x = torch.randn(V, generator=g)
+        x[torch.randperm(V, generator=g)[:n]] = math.nan
+        rows.append(x)
+    x = torch.stack(rows)
+    for dtype in TYPES:
+        y = x.to(dtype)
+        got = L().top_logits(y.cuda().repeat(times, 1), k)
+        got = [t.view(times, len(rows), *t.shape[1:]) for t in got]
+        for t in got:
+            bits = t.view(torch.int32) if t.dtype == torch.float32 else t
+            assert bool((bits == bits[:1]).all())
+        for i in range(len(rows)):  # (one at a time: the tolerance is that of a row's own range)
+            check_top(y[i:i + 1], k, 1.0, got=[t[0, i:i + 1] for t in got])
+
+
 @pytest.mark.parametrize("V", [9001, 40000, 200001])
 def test_top_logits_where_the_others_lie_far_below(V):
     """The k-th value is far above everything that is left, in the whole row or in one stretch of it only."""
@@ -543,10 +572,30 @@ def test_distill_factors_and_second_walks():
     loss = L().DistillLoss(2.0, 0.5)(leaf, **dev)
     with torch.no_grad():
         leaf += 1
-    with pytest.raises(RuntimeError, match="in place"):
+    with pytest.raises(RuntimeError, match="in ?place"):
         loss.backward()
     with pytest.raises(SpeechAmdError, match="once"):
         torch.autograd.grad(L().DistillLoss(2.0, 0.5)(leaf, **dev), leaf, create_graph=True)
+    for name in ("values", "ids", "rest", "targets", "weights"):
+        mine = {a: v.clone() for a, v in dev.items()}
+        loss = L().DistillLoss(2.0, 0.5)(leaf, **mine)
+        mine[name].zero_()
+        with pytest.raises(RuntimeError, match="in place"):
+            (2 * loss).backward()
+    # the walk frees the logits, and says so to a second one
+    loss = L().DistillLoss(2.0, 0.5)(leaf, **dev)
+    (2 * loss).backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        (2 * loss).backward()
+    # what a teacher made in inference mode is as good as any other
+    with torch.inference_mode():
+        given = {a: v.clone() for a, v in dev.items()}
+        L().constrain(leaf, bias_ids=dev["ids"], bias_values=dev["values"])
+    leaf.grad = None
+    (2 * L().DistillLoss(2.0, 0.5)(leaf, **given)).backward()
+    by_lists, leaf.grad = leaf.grad, None
+    (2 * L().DistillLoss(2.0, 0.5)(leaf, **dev)).backward()
+    assert torch.equal(by_lists, leaf.grad)
 
 
 def test_distill_gradient_against_differences():

@@ -127,6 +127,14 @@ def test_the_c_entries_refuse_before_they_launch():
     assert dis(k=0) == dis(k=129) == dis(t=0.0) == dis(t=math.nan) == dis(alpha=1.5) == dis(alpha=math.nan) == bad
     assert top(t=1e-9) == top(t=1e9) == dis(t=1e-9) == dis(t=1e9) == bad
     assert dis(x=None) == dis(rows=-1) == dis(loss_rows=None) == dis(loss=None, dx=None) == dis(V=0) == bad
+    # more rows than a launch has threads for
+    assert top(rows=1 << 28) == top(rows=1 << 27, V=100) == top(rows=1 << 26, V=500) == top(rows=1 << 40) == bad
+    assert dis(rows=1 << 26) == dis(rows=1 << 24, V=5000) == dis(rows=1 << 40) == bad
+    assert lib.sa_top_logits_workspace_bytes(1 << 40, 8, 2, 0) == 0
+    c = _lib.saConstraints()
+    ref = ctypes.byref(c)
+    assert lib.sa_logits_pick(P, 8, 0, 1 << 24, 8, ref, P, P, None, 0, None) == bad
+    assert lib.sa_logits_constrain(P, 8, 0, P, 8, 1 << 24, 8, ref, None) == bad
 
 
 def test_the_constrained_decode_refuses_before_it_launches():
