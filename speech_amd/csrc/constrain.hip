@@ -66,12 +66,12 @@ template <int VEC> __device__ __forceinline__ unsigned con_allowed(const unsigne
     return (unsigned)(((((unsigned long long)b) << 32 | a)) >> (v0 & 31));
 }
 
-template <typename T, int NV, bool PICK>
-__global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T* y /* may be x */, long ldy, int V, int nseg, int per,
+template <typename T, int NT, int NV, bool PICK>
+__global__ __launch_bounds__(NT) void constrain_kernel(const T* x, long ldx, T* y /* may be x */, long ldy, int V, int nseg, int per,
                                                         saConstraints C, PickPart* __restrict__ part, long long* __restrict__ tokens,
                                                         float* __restrict__ logp) {
-    constexpr int VEC = SaVec<T>::N, NT = 256, SEG = NT * NV * VEC;
-    extern __shared__ uint4 words4[];  // SEG words, then SEG positions (16 bits); nothing where there are no lists
+    constexpr int VEC = SaVec<T>::N, SEG = NT * NV * VEC;
+    extern __shared__ uint4 words4[];  // SEG words, then a position (16 bits) an entry, SEG at most; nothing where there are no lists
     __shared__ int found;
     __shared__ PickPart waves[NT / 64];
     unsigned* const words = (unsigned*)words4;
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256) void constrain_kernel(const T* x, long ldx, T*
     const int first = seg * per * VEC - sa_lead(xr), end = first + per * VEC < V ? first + per * VEC : V;
     // Everything the row needs from memory is asked for at once, the lists first: their atomics are the longer way.
     const bool lists = C.history || C.bias_ids;
-    constexpr int AHEAD = 8;  // history entries a thread has in flight (2048 a workgroup)
+    constexpr int AHEAD = 8;  // history entries a thread has in flight
     long long past[AHEAD], biased = -1;
     const long long* h = C.history + (long)row * C.history_ld;
     const long long* ids = C.bias_ids + (long)row * C.bias_ld;
@@ -238,18 +238,22 @@ __global__ __launch_bounds__(64) void pick_join_kernel(const PickPart* __restric
     if (threadIdx.x == 0) pick_write(r, tokens + blockIdx.x, logp + blockIdx.x);
 }
 
-// Vectors a thread, segments a row, vectors a segment.  Segments of 4096 tokens -- each reads the lists of its row again, and three
-// times as many of them run on a CU as of 8192 (256 x 131072 f32: 71 us; 8192 tokens 85, 2048 tokens 82) -- and shorter ones where
-// that leaves CUs without work.  Where it saves pick its second launch, one workgroup takes a row of up to 8192.
-struct ConPlan { int nv, nseg, per; };
-ConPlan con_plan(int rows, int V, int dtype, bool pick) {
+// Threads, vectors a thread, segments a row, vectors a segment.  Segments of 4096 tokens -- each reads the lists of its row again,
+// and three times as many of them run on a CU as of 8192 by the same 256 threads (256 x 131072 f32, history 4096: 71 us; 8192 tokens
+// 85, 2048 tokens 82) -- and shorter ones where that leaves CUs without work.  Long lists are worth 512 threads and 8192 tokens, half
+// as many looks at the lists by as many waves (61 -> 52 us with everything in the caches, history 1500 45 -> 44, 65535 365 -> 253;
+// 1024 threads 56, 45, 236), where three of those workgroups come to every CU.  Where it saves pick its second launch, one workgroup
+// takes a row of up to 8192.
+struct ConPlan { int nt, nv, nseg, per; };
+ConPlan con_plan(int rows, int V, int dtype, bool pick, int entries) {
     const int vec = dtype == SA_F32 ? 4 : 8, most = 16 / vec, vectors = (V + 2 * vec - 2) / vec;
-    ConPlan p{1, 1, 0};
+    ConPlan p{256, 1, 1, 0};
     const bool whole = pick && vectors <= 512 * most;
     while (256 * p.nv < vectors &&
            (whole || (p.nv < most && (long)rows * ((vectors + 512 * p.nv - 1) / (512 * p.nv)) >= 512)))
         p.nv *= 2;
-    p.nseg = (vectors + 256 * p.nv - 1) / (256 * p.nv);
+    if (!pick && entries > 1024 && vectors > 256 * most && (long)rows * ((vectors + 512 * most - 1) / (512 * most)) >= 768) p.nt = 512;
+    p.nseg = (vectors + p.nt * p.nv - 1) / (p.nt * p.nv);
     p.per = (vectors + p.nseg - 1) / p.nseg;
     p.nseg = (vectors + p.per - 1) / p.per;
     return p;
@@ -275,15 +279,18 @@ template <typename T, bool PICK>
 void con_launch(const void* x, long ldx, void* y, long ldy, int rows, int V, const ConPlan& p, const saConstraints& c,
                 PickPart* part, long long* tokens, float* logp, hipStream_t stream) {
     const saConstraints C = con_used(c);
-    const dim3 grid((unsigned)((size_t)rows * p.nseg)), block(256);
-    const size_t smem = C.history || C.bias_ids ? (size_t)256 * p.nv * SaVec<T>::N * 6 : 0;
-#define CON_LAUNCH(NV)                                                                                                        \
-    hipLaunchKernelGGL((constrain_kernel<T, NV, PICK>), grid, block, smem, stream, (const T*)x, ldx, (T*)y, ldy, V, p.nseg, p.per, \
+    const dim3 grid((unsigned)((size_t)rows * p.nseg)), block(p.nt);
+    const size_t segment = (size_t)p.nt * p.nv * SaVec<T>::N, entries = (size_t)c.history_len + c.n_bias;
+    const size_t smem = entries ? segment * 4 + (entries < segment ? entries : segment) * 2 : 0;
+#define CON_LAUNCH(NT, NV)                                                                                                        \
+    hipLaunchKernelGGL((constrain_kernel<T, NT, NV, PICK>), grid, block, smem, stream, (const T*)x, ldx, (T*)y, ldy, V, p.nseg, p.per, \
                        C, part, tokens, logp)
-    if (p.nv == 1) CON_LAUNCH(1);
-    else if (p.nv == 2) CON_LAUNCH(2);
-    else if (p.nv == 4) CON_LAUNCH(4);
-    else if constexpr (PICK && sizeof(T) == 4) CON_LAUNCH(8);
+    if (p.nt == 512) {
+        if constexpr (!PICK) CON_LAUNCH(512, 16 / SaVec<T>::N);
+    } else if (p.nv == 1) CON_LAUNCH(256, 1);
+    else if (p.nv == 2) CON_LAUNCH(256, 2);
+    else if (p.nv == 4) CON_LAUNCH(256, 4);
+    else if constexpr (PICK && sizeof(T) == 4) CON_LAUNCH(256, 8);
 #undef CON_LAUNCH
 }
 
@@ -302,8 +309,8 @@ extern "C" ctcStatus_t sa_logits_constrain(const void* x, long ldx, int dtype, v
     SA_CLEAR_ERR();
     if (rows < 0 || !sa_rows_ok(dtype, V) || !con_ok(c, rows, V)) return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
-    const ConPlan p = con_plan(rows, V, dtype, false);
-    if (!x || !y || !sa_threads_ok((long)rows * p.nseg, 256)) return CTC_STATUS_INVALID_VALUE;
+    const ConPlan p = con_plan(rows, V, dtype, false, c->history_len + c->n_bias);
+    if (!x || !y || !sa_threads_ok((long)rows * p.nseg, p.nt)) return CTC_STATUS_INVALID_VALUE;
     con_run<false>(x, ldx, dtype, y, ldy, rows, V, p, *c, nullptr, nullptr, nullptr, (hipStream_t)stream);
     SA_CHECK_LAUNCH();
     return CTC_STATUS_SUCCESS;
@@ -311,7 +318,7 @@ extern "C" ctcStatus_t sa_logits_constrain(const void* x, long ldx, int dtype, v
 
 extern "C" size_t sa_logits_pick_workspace_bytes(int rows, int V, int dtype) {
     if (rows < 1 || !sa_rows_ok(dtype, V)) return 0;
-    const ConPlan p = con_plan(rows, V, dtype, true);
+    const ConPlan p = con_plan(rows, V, dtype, true, 0);
     return p.nseg == 1 ? 0 : (size_t)rows * p.nseg * sizeof(PickPart);
 }
 
@@ -321,7 +328,7 @@ extern "C" ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int ro
     SA_CLEAR_ERR();
     if (rows < 0 || !sa_rows_ok(dtype, V) || !con_ok(c, rows, V)) return CTC_STATUS_INVALID_VALUE;
     if (rows == 0) return CTC_STATUS_SUCCESS;
-    const ConPlan p = con_plan(rows, V, dtype, true);
+    const ConPlan p = con_plan(rows, V, dtype, true, 0);
     const size_t need = sa_logits_pick_workspace_bytes(rows, V, dtype);
     if (!x || !d_tokens || !d_logp || (need && (!workspace || workspace_bytes < need)) || !sa_threads_ok((long)rows * p.nseg, 256))
         return CTC_STATUS_INVALID_VALUE;

@@ -69,7 +69,9 @@ SHAPES = [(1, 1, 0, 0, True), (2, 29, 40, 3, True), (32, 29, 200, 0, True), (3, 
           (3, 4095, 300, 20, True), (2, 4096, 5000, 0, False), (4, 4097, 64, 64, True), (3, 8193, 600, 10, True), (2, 16385, 1, 1, True),
           (2, 32000, 1500, 128, True), (7, 50021, 333, 16, True), (2, 131072, 4096, 100, True), (1, 262147, 70, 5, False),
           (1, 1048576, 900, 300, True), (1, 1044481, 64, 0, False), (130, 8190, 20, 2, True),
-          (600, 8190, 9, 3, True)]
+          (600, 8190, 9, 3, True),
+          # long lists and enough rows for larger workgroups; one entry too few for them
+          (800, 5000, 1100, 40, True), (160, 40003, 3000, 0, False), (258, 16385, 1000, 25, True), (258, 16385, 1000, 24, True)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
