@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import SpeechAmdError, check
+from .ops import is_unit_gradient
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 VOCAB_MAX, LIST_MAX, TOP_MAX = 1048576, 65535, 128
@@ -57,7 +58,7 @@ def _rows_of(x, name="logits"):
 
 def _tensor(t, name, dtype, shape, device):
     """The device pointer of a packed tensor of exactly this type, shape and device."""
-    if not torch.is_tensor(t) or t.dtype != dtype or tuple(t.shape) != tuple(shape):
+    if not torch.is_tensor(t) or t.dtype != dtype or t.shape != shape:
         raise SpeechAmdError("%s must be a %s tensor of shape %s" % (name, dtype, tuple(shape)))
     if t.device != device:
         raise SpeechAmdError("%s must be on %s like the logits, not %s" % (name, device, t.device))
@@ -259,7 +260,10 @@ def top_logits(logits, k, temperature=1.0):
 
 def _versions(tensors):
     """How often each has been written to (a tensor made in inference mode does not count that)."""
-    return [None if t is None or t.is_inference() else t._version for t in tensors]
+    try:
+        return [t._version for t in tensors]
+    except RuntimeError:
+        return [None if t.is_inference() else t._version for t in tensors]
 
 
 class DistillFunction(torch.autograd.Function):
@@ -291,13 +295,13 @@ class DistillFunction(torch.autograd.Function):
             # six of its records cost more than the launches)
             ctx.save_for_backward(x)
             lists = (values, ids, rest, targets, weights)
-            ctx.again = (lists, _versions(lists), ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale)
+            given = [t for t in lists if t is not None]
+            ctx.again = (lists, given, _versions(given), ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale)
             ctx.dx = dx
         return loss
 
     @staticmethod
     def backward(ctx, go):
-        from .ops import is_unit_gradient
         if torch.is_grad_enabled():
             raise SpeechAmdError("the distillation loss is differentiable once: its gradient is no function of the logits to autograd")
         # the first walk takes the buffer of the forward pass along: it is handed out once and never written again
@@ -305,17 +309,16 @@ class DistillFunction(torch.autograd.Function):
         if dx is not None and is_unit_gradient(go):
             return dx, None, None, None, None, None, None, None, None
         x, = ctx.saved_tensors
-        lists, versions, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale = ctx.again
-        if _versions(lists) != versions:
+        lists, given, versions, ld_outer, ld_inner, n_inner, rows, V, k, temperature, alpha, scale = ctx.again
+        if _versions(given) != versions:
             raise RuntimeError("the teacher's list, targets or weights of a distillation loss were changed in place after its forward pass")
-        values, ids, rest, targets, weights = lists
         fresh = dx is None
         if fresh:
             dx = torch.empty_like(x)
-        factor = go.reshape(1).to(torch.float32)
-        p = _lib.ptr
-        _launch("sa_distill_loss", x, p(x), p(dx), ld_outer, ld_inner, n_inner, _DTYPES[x.dtype], rows, V, p(values), p(ids), p(rest), k,
-                p(targets), p(weights), temperature, alpha, scale, p(factor), 0 if fresh else 1, None, None)
+        values, ids, rest, targets, weights = [None if t is None else t.data_ptr() for t in lists]
+        # (go: one float32, the type and shape of the loss)
+        _launch("sa_distill_loss", x, x.data_ptr(), dx.data_ptr(), ld_outer, ld_inner, n_inner, _DTYPES[x.dtype], rows, V, values, ids,
+                rest, k, targets, weights, temperature, alpha, scale, go.data_ptr(), 0 if fresh else 1, None, None)
         return dx, None, None, None, None, None, None, None, None
 
 
