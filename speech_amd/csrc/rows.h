@@ -84,6 +84,10 @@ template <> __device__ __forceinline__ unsigned sa_fill_word<float>() { return 0
 template <> __device__ __forceinline__ unsigned sa_fill_word<SaBf16>() { return 0xff80ff80u; }
 template <> __device__ __forceinline__ unsigned sa_fill_word<SaF16>() { return 0xfc00fc00u; }
 
+__device__ __forceinline__ unsigned sa_bits(float x) { return __builtin_bit_cast(unsigned, x); }
+__device__ __forceinline__ unsigned sa_bits(SaBf16 x) { return x.v; }
+__device__ __forceinline__ unsigned sa_bits(SaF16 x) { return x.v; }
+
 template <typename T> __device__ __forceinline__ int sa_lead(const T* row) { return (int)(((uintptr_t)row & 15) / sizeof(T)); }
 
 template <typename T> __device__ __forceinline__ float sa_element(const uint4& q, int e);
@@ -140,24 +144,47 @@ template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v
         if (v0 + e >= 0 && v0 + e < V) row[v0 + e] = sa_narrow<T>(g[e]);
 }
 
-// the vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V)
-template <typename T> __device__ __forceinline__ uint4 sa_load_vec(const T* row, int v0, int V) {
+// The vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V).  A row's first and last vector: all their
+// elements at once, those outside taken from the row's ends and dropped -- one wait, where one element after the other costs rows of
+// odd lengths 10 - 20 % (8000 x 5001 bf16: top logits 48 -> 42 us, constrain 52 -> 43, distillation 54 -> 48).  TIGHT: one after the
+// other after all, for kernels without the registers (top logits, 4096 x 32000 bf16: 71 us against 78).
+template <typename T, bool TIGHT = false> __device__ __forceinline__ uint4 sa_load_vec(const T* row, int v0, int V) {
     if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
-    // (a loop and not eight copies of its body: a row has two such vectors, and the registers of the others are wanted)
-    constexpr int BITS = 8 * (int)sizeof(T);
-    const unsigned long long f = (unsigned long long)sa_fill_word<T>() << 32 | sa_fill_word<T>();
-    unsigned long long w[2] = {f, f};
+    constexpr int N = SaVec<T>::N, BITS = 8 * (int)sizeof(T);
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = sa_fill_word<T>();
+    if (v0 >= V) return make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (TIGHT) {
+        unsigned long long u[2] = {(unsigned long long)w[1] << 32 | w[0], (unsigned long long)w[3] << 32 | w[2]};
 #pragma unroll 1
-    for (int e = 0; e < SaVec<T>::N; ++e) {
-        const int v = v0 + e;
-        if (v < 0 || v >= V) continue;
-        unsigned long long h;
-        if constexpr (sizeof(T) == 4) h = __builtin_bit_cast(unsigned, row[v]);
-        else h = __builtin_bit_cast(sa_u16, row[v]);
-        const int at = e * BITS & 63;
-        const unsigned long long keep = ~(((1ull << BITS) - 1) << at);
-        if (e * BITS < 64) w[0] = (w[0] & keep) | h << at;
-        else w[1] = (w[1] & keep) | h << at;
+        for (int e = 0; e < N; ++e) {
+            const int v = v0 + e;
+            if (v < 0 || v >= V) continue;
+            const unsigned long long h = sa_bits(row[v]);
+            const int at = e * BITS & 63;
+            const unsigned long long keep = ~(((1ull << BITS) - 1) << at);
+            if (e * BITS < 64) u[0] = (u[0] & keep) | h << at;
+            else u[1] = (u[1] & keep) | h << at;
+        }
+        return make_uint4((unsigned)u[0], (unsigned)(u[0] >> 32), (unsigned)u[1], (unsigned)(u[1] >> 32));
+    } else {
+        unsigned h[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int v = v0 + e;
+            h[e] = sa_bits(row[v < 0 ? 0 : v >= V ? V - 1 : v]);
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int v = v0 + e;
+            if constexpr (BITS == 32) {
+                w[e] = v >= 0 && v < V ? h[e] : w[e];
+            } else {
+                const unsigned u = v >= 0 && v < V ? h[e] : sa_fill_word<T>() & 0xffffu;
+                w[e / 2] = e & 1 ? w[e / 2] | u << 16 : u;
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    return make_uint4((unsigned)w[0], (unsigned)(w[0] >> 32), (unsigned)w[1], (unsigned)(w[1] >> 32));
 }

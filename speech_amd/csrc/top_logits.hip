@@ -165,9 +165,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
     const int first = seg * per * VEC - sa_lead(xr);  // the segment's first element (may lie before the row)
     const int end = first + per * VEC < V ? first + per * VEC : V;
     const float c = SA_LOG2E / temperature;
+    constexpr bool TIGHT = NV * VEC > 32;
     uint4 raw[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec(xr, first + (i * NT + tid) * VEC, end);
+    for (int i = 0; i < NV; ++i) raw[i] = sa_load_vec<T, TIGHT>(xr, first + (i * NT + tid) * VEC, end);
     const int lo = first < 0 ? 0 : first, valid = end > lo ? end - lo : 0;
 
     float mx = -INFINITY;
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
             for (int i = 0; i < NV; ++i) {
                 const int v0 = first + (i * NT + tid) * VEC;
                 if (v0 >= until) break;
-                const uint4 r = sa_load_vec(xr, v0, end);
+                const uint4 r = sa_load_vec<T, TIGHT>(xr, v0, end);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e)
                     if (v0 + e >= lo && v0 + e < until) visit(sa_element<T>(r, e), v0 + e);
