@@ -182,6 +182,16 @@ def _matrix(logits):
     return ld, rows, logits.shape[1]
 
 
+def _overlap(x, ldx, y, ldy, rows, V):
+    """Whether two (rows, V) matrices of one type share elements without being the same matrix."""
+    off = (y.data_ptr() - x.data_ptr()) // x.element_size()
+    if rows == 0 or (off == 0 and (ldx == ldy or rows == 1)):
+        return False
+    if off >= (rows - 1) * ldx + V or -off >= (rows - 1) * ldy + V:
+        return False
+    return rows == 1 or ldx != ldy or off % ldx < V or -off % ldx < V  # (columns of one matrix may lie beside each other)
+
+
 def constrain(logits, history=None, lengths=None, repetition=None, presence=None, frequency=None, bias_ids=None,
               bias_values=None, mask=None, states=None, out=None):
     """The logits (requests, V) of each request's next token under its constraints, in the logits' type.
@@ -203,6 +213,8 @@ def constrain(logits, history=None, lengths=None, repetition=None, presence=None
         ldo, _, _, _ = _rows_of(out, "out")
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (rows > 1 and ldo < V):
             raise SpeechAmdError("out must be like the logits, without overlapping rows")
+        if _overlap(logits, ld, out, ldo, rows, V):
+            raise SpeechAmdError("out must be the logits themselves or share nothing with them")
         if out.requires_grad and torch.is_grad_enabled():
             raise SpeechAmdError("constrain writes to out without recording it: out must not require a gradient")
     torch.autograd.graph.increment_version(out)  # (written behind autograd's back: whoever saved it must see that)

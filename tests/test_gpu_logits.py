@@ -203,6 +203,11 @@ def test_constrain_refuses_on_the_gpu():
                dict(out=torch.zeros(1, 40).cuda().expand(3, 40)), dict(out=torch.zeros(3, 40).cuda().requires_grad_())):
         with pytest.raises(SpeechAmdError):
             L().constrain(x, **kw)
+    wide = torch.zeros(4, 80).cuda()
+    with pytest.raises(SpeechAmdError, match="share"):
+        L().constrain(wide[:3], out=wide[1:])
+    L().constrain(wide[:, :40], bias_ids=torch.zeros(4, 1, dtype=torch.int64).cuda(), bias_values=torch.ones(4, 1).cuda(), out=wide[:, 40:])
+    assert wide[:, 40].tolist() == [1.0] * 4 and float(wide.abs().sum()) == 4.0
     with pytest.raises(SpeechAmdError):
         L().pick(torch.zeros(2, 3, 40).cuda())
     seen = x._version   # written in place: whoever saved the tensor must see that

@@ -154,6 +154,19 @@ def test_the_constrained_decode_refuses_before_it_launches():
     assert run(states=None) == bad
 
 
+def test_what_out_may_share_with_the_logits():
+    b = torch.zeros(6, 10)
+
+    def meet(x, y):
+        return L._overlap(x, x.stride(0), y, y.stride(0), x.shape[0], x.shape[1])
+    assert not meet(b, b) and not meet(b, b.clone()) and not meet(b[:3], b[3:]) and not meet(b[3:], b[:3])
+    assert not meet(b[:, :5], b[:, 5:]) and not meet(b[:, 5:], b[:, :5]) and not meet(b[::2], b[1::2])
+    assert not meet(b[:, :4], b[:, 6:]) and not meet(b[:1], b[:1]) and not meet(b[:0], b[:0])
+    assert meet(b[:4], b[1:5]) and meet(b[1:5], b[:4]) and meet(b[:, :6], b[:, 4:]) and meet(b[:, 4:], b[:, :6])
+    assert meet(b[:2, :5], b[::2][:2, :5]) and meet(b[:1].expand(3, 10), b[:3]) and meet(b.view(1, 60)[:, :20], b.view(1, 60)[:, 10:30])
+    assert meet(b[:3, :8], b.as_strided((3, 8), (10, 1), 13))
+
+
 def test_pack_mask():
     g = torch.Generator().manual_seed(3)
     for V in (1, 31, 32, 33, 64, 100):
