@@ -267,6 +267,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
         }
     }
     s = sa_block_sum<NT / 64>(s, sums);
+    if constexpr (NT == 64) __syncthreads();  // (one wave sums without a barrier)
     int C = count;
     float m = b;
     if (C > cap || (C < valid && !(s >= 0x1p-70f && s <= 2.0f * valid))) {
@@ -320,6 +321,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void to
         }
         const float t = number(K);
         auto taken = [&](float f, int v) __attribute__((always_inline)) { return f > t || (f != f && t == t) || ((f == t || (f != f && t != t)) && v < places); };
+        __syncthreads();  // (nobody still has to read the first count: where it fits, no look at the row came in between)
         if (tid == 0) count = 0;
         __syncthreads();
         float most = -INFINITY;

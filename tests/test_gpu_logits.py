@@ -327,6 +327,29 @@ def test_top_logits_where_the_others_lie_far_below(V):
             check_top(x[row:row + 1].to(dtype), k, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("n,V", [(1100, 900), (600, 1000), (600, 2000), (300, 4000), (300, 8000), (300, 16000), (260, 32000), (40, 40000),
+                                 (3, 300007)])
+def test_top_logits_that_stand_out_in_every_kernel_form(n, V, dtype):
+    """A few more than k tokens stand out and the others vanish beside them: the candidates fit at once, and the row is looked at again
+    for the others' sum alone.  Every form of the kernel (a wave, 256 to 1024 threads, segments), the top scattered or in one stretch;
+    the lists and the bits of every run are the same."""
+    g = gen(n + V)
+    k = 40
+    for fill in (-math.inf, -200.0):
+        x = torch.full((n, V), fill)
+        for b in range(n):
+            many = k + 7 * (b % 5)
+            at = torch.randperm(V, generator=g)[:many] if b % 2 else torch.randint(0, V - 2 * k, (1,), generator=g) + torch.randperm(2 * k, generator=g)[:many]
+            x[b, at] = torch.randn(many, generator=g) * 3 + 50
+        x = x.to(dtype)
+        dev = x.cuda()
+        want = L().top_logits(dev, k)
+        check_top(x, k, got=want)
+        for _ in range(4):
+            assert all(torch.equal(a, b) for a, b in zip(L().top_logits(dev, k), want))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("V", [29, 5001, 33000])
 def test_top_logits_of_views(V, dtype):
