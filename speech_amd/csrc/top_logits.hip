@@ -438,20 +438,21 @@ __global__ __launch_bounds__(NT) void top_merge_kernel(const unsigned long long*
     if (left) m = fmaxf(m, sa_unorder((unsigned)(left >> 32)));
     m = sa_block_max<NT / 64>(m, sums);
     float s = sa_block_sum<NT / 64>(P.s != 0.0f ? P.s * top_exp(P.m, m, c) : 0.0f, sums);
-    // The lists are in the order of arrival: their terms (0 .. 1) are summed as integers of 2^-32, the same in any order.
+    // The lists are in the order of arrival: their terms (0 .. 1) are rounded to multiples of 2^-48 and summed as integers, the same in
+    // any order.  28896 terms at most: the sum stays below 2^63, and all roundings together below 2^-34 of a sum of 1 or more.
     unsigned long long sum = 0;
     if (left) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
             if (keys[i] && keys[i] < last) {
                 const float e = top_exp(sa_unorder((unsigned)(keys[i] >> 32)), m, c);
-                if (e == e) sum += (unsigned long long)(e * 0x1p32f);
+                if (e == e) sum += __float2ull_rn(e * 0x1p48f);
                 else odd = 1;
             }
     }
     if (sum) atomicAdd(&total, sum);
     __syncthreads();
-    s += odd ? NAN : (float)total * 0x1p-32f;
+    s += odd ? NAN : (float)total * 0x1p-48f;
     if (tid == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 

@@ -350,6 +350,27 @@ def test_top_logits_that_stand_out_in_every_kernel_form(n, V, dtype):
             assert all(torch.equal(a, b) for a, b in zip(L().top_logits(dev, k), want))
 
 
+@pytest.mark.parametrize("n,V,k", [(8, 131071, 100), (2, 300007, 128), (1, 1048576, 128)])
+def test_top_logits_with_a_long_list_of_small_terms(n, V, k):
+    """One token of the others stands at 0 and thousands at -22.4, below 2^-32 of it each, in the lists that long rows are joined from:
+    together they are up to 70 * 2^-24 of the sum.  The sum S is 1 and a little: each of the two roundings of a float32 sum there is half
+    a step of [1, 2), 2^-24; log(S) and the small terms themselves are off by less than 2^-24 of a few 2^-19; in all 4 * 2^-24."""
+    g = gen(V)
+    x = torch.full((n, V), -40.0)
+    step = 7000                                       # less than any segment of such rows
+    for b in range(n):
+        for at in range(0, V - step + 1, step):
+            x[b, at + torch.randperm(step, generator=g)[:150]] = -22.4
+        at = torch.randperm(step, generator=g)[:k + 1]
+        x[b, at[:k]] = 10.0 + torch.arange(k) / 16
+        x[b, at[k]] = 0.0
+    _, ids, rest = L().top_logits(x.cuda(), k)
+    _, wi, wr = ref.top_logits(x, k)
+    assert torch.equal(ids.cpu(), wi)
+    assert float((wr - (x == -22.4).sum(1) * math.exp(-22.4)).abs().max()) < 1e-8    # (the list is what counts beside the 1)
+    assert float((rest.cpu().double() - wr).abs().max()) <= 4 * U
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("V", [29, 5001, 33000])
 def test_top_logits_of_views(V, dtype):
