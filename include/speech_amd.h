@@ -630,6 +630,7 @@ ctcStatus_t sa_top_logits(const void* x, long ld_outer, long ld_inner, int n_inn
  *     soft = sum_j q_j (log q_j - log p_id(j))  [+ q_rest (log q_rest - log p_rest)]     (0 for a row without entries)
  *     hard = log sum exp(x) - x[target]                                    (0 for a target outside [0, V), or targets NULL)
  *     loss_rows[i] = scale * weights[i] * (alpha * temperature^2 * soft + (1 - alpha) * hard);   *loss = their sum
+ * NaN or +inf among a row's entries or in its rest is no distribution: that row's loss is NaN (unless alpha or its weight is 0).
  * A row of weight 0 is not read: its loss and its gradient are 0 whatever it holds.  weights NULL: 1.
  * dx (the layout of x, no part of it shared with x, or NULL) = the gradient of *loss with respect to x, times *d_factor when d_factor != NULL.
  * loss == NULL: only the gradient; then skip_unit != 0 leaves dx untouched when *d_factor is 1 (dx holds it already).

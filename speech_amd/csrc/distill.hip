@@ -116,7 +116,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
     if (tid < 64) {
         if (REST) ar = A.rest[row];
         am = fmaxf(sa_wave_max_dpp(fmaxf(a[0], a[1])), ar);
-        soft = am > -INFINITY && A.alpha > 0.0f;
+        // (a list that holds NaN, or +inf, has no distribution: q, the loss and the list's gradients become NaN, whatever else is there)
+        soft = (am > -INFINITY || __any(a[0] != a[0] || a[1] != a[1] || ar != ar)) && A.alpha > 0.0f;
         const float e0 = soft ? sa_exp2((a[0] - am) * SA_LOG2E) : 0.0f, e1 = soft ? sa_exp2((a[1] - am) * SA_LOG2E) : 0.0f;
         const float er = soft && REST ? sa_exp2((ar - am) * SA_LOG2E) : 0.0f;
         const float total = sa_wave_sum_dpp(e0 + e1) + er;
@@ -260,10 +261,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T*
         float l = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (q[i] > 0.0f) l += q[i] * ((a[i] - am) - lt - ((xv[i] - m) / A.temperature - lS));
+            if (q[i] != 0.0f) l += q[i] * ((a[i] - am) - lt - ((xv[i] - m) / A.temperature - lS));
         l = sa_wave_sum_dpp(l);
         if (lane == 0) {
-            if (REST && qr > 0.0f) l += qr * ((ar - am) - lt - ((mr - m) / A.temperature + logf(sr) - lS));
+            if (REST && qr != 0.0f) l += qr * ((ar - am) - lt - ((mr - m) / A.temperature + logf(sr) - lS));
             float v = soft ? A.alpha * A.temperature * A.temperature * l : 0.0f;
             if (hard) v += (1.0f - A.alpha) * (logf(H) - (xt - m));
             A.loss_rows[row] = f * v;

@@ -345,8 +345,8 @@ class DistillLoss(torch.nn.Module):
 
     forward(logits (..., V), values (..., k) float32, ids (..., k) int64, rest=None (...) float32, targets=None (...) int64,
     weights=None (...) float32) -> (1,) float32.  An id that is no class is absent from the list (padding), a target that is none
-    gives no hard term, a row of weight 0 is not read and has a gradient of 0 whatever it holds.  Only the logits get a gradient,
-    in their own type; it is differentiable once."""
+    gives no hard term, a row of weight 0 is not read and has a gradient of 0 whatever it holds; NaN or +inf in another row's list or
+    rest makes the loss NaN.  Only the logits get a gradient, in their own type; it is differentiable once."""
 
     def __init__(self, temperature=1.0, alpha=1.0, denom=None):
         super().__init__()

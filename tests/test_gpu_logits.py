@@ -539,6 +539,40 @@ def test_distill_of_rows_that_are_not_ordinary(V):
     assert float((leaf.grad.cpu().double() - wg).abs().max()) <= 300 * U
 
 
+@pytest.mark.parametrize("V", [29, 700, 9000, 40000, 140000])
+def test_distill_of_a_teacher_that_is_no_distribution(V):
+    """NaN or +inf among the entries or in the rest: the loss says so, and every other row's gradient is as ever."""
+    g = gen(V)
+    n, k = 4, 6
+    x, kw = student(g, n, V, torch.float32, k, 2.0, weights=False)
+    clean = x.cuda().requires_grad_(True)
+    L().DistillLoss(2.0, 0.6)(clean, **cuda(kw)).backward()
+    for bad in (math.nan, math.inf):
+        for where in ("values", "rest", "only entry", "without a rest"):
+            mine = {a: t.clone() for a, t in kw.items()}
+            if where == "rest":
+                mine["rest"][1] = bad
+            else:
+                mine["values"][1, 3] = bad
+            if where == "only entry":
+                mine["ids"][1, :3] = mine["ids"][1, 4:] = -1
+                mine["rest"][1] = -math.inf
+            if where == "without a rest":
+                mine["rest"] = None
+                mine["ids"][1, :3] = mine["ids"][1, 4:] = -1
+            leaf = x.cuda().requires_grad_(True)
+            loss = L().DistillLoss(2.0, 0.6)(leaf, **cuda(mine))
+            loss.backward()
+            assert bool(loss.detach().isnan()), (bad, where)
+            assert bool(leaf.grad[1, mine["ids"][1, 3].item()].isnan()), (bad, where)
+            if where != "without a rest":
+                assert torch.equal(leaf.grad[[0, 2, 3]], clean.grad[[0, 2, 3]]), (bad, where)
+            w = torch.ones(n)
+            w[1] = 0.0
+            assert bool(L().DistillLoss(2.0, 0.6)(leaf.detach(), weights=w.cuda(), **cuda(mine)).isfinite())
+            assert bool(L().DistillLoss(2.0, 0.0)(leaf.detach(), **cuda(mine)).isfinite())
+
+
 def test_distill_rows_without_anything():
     """No entry, no rest, no target: no loss and a gradient of exactly zero."""
     x = torch.randn(4, 50, generator=gen(1)).cuda().requires_grad_(True)
