@@ -261,8 +261,9 @@ ConPlan con_plan(int rows, int V, int dtype, bool pick, int entries) {
 
 bool con_ok(const saConstraints* c, int rows, int V) {
     if (!c || c->history_len < 0 || c->history_len > SA_LIST_MAX || c->n_bias < 0 || c->n_bias > SA_LIST_MAX) return false;
-    if (c->history_len > 0 && (!c->history || c->history_ld < 0)) return false;
-    if (c->n_bias > 0 && (!c->bias_ids || !c->bias_values || c->bias_ld < 0)) return false;
+    // (without a request nothing is read: an empty list has no address)
+    if (c->history_len > 0 && ((rows > 0 && !c->history) || c->history_ld < 0)) return false;
+    if (c->n_bias > 0 && ((rows > 0 && (!c->bias_ids || !c->bias_values)) || c->bias_ld < 0)) return false;
     if (c->mask && (c->n_states < 1 || c->mask_ld < (V + 31) / 32 || (!c->states && c->n_states < rows))) return false;
     return true;
 }

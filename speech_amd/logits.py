@@ -88,7 +88,7 @@ def pack_mask(allowed):
     if not torch.is_tensor(allowed) or allowed.dtype != torch.bool or allowed.dim() != 2 or allowed.shape[1] < 1:
         raise SpeechAmdError("a mask is packed from a (states, V) bool tensor")
     n, v = allowed.shape
-    bits = torch.nn.functional.pad(allowed, (0, -v % 32)).view(n, -1, 32).to(torch.int64)
+    bits = torch.nn.functional.pad(allowed, (0, -v % 32)).view(n, (v + 31) // 32, 32).to(torch.int64)
     words = (bits << torch.arange(32, device=allowed.device)).sum(2)
     return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
 
@@ -138,7 +138,7 @@ def _constraints(rows, V, dev, history, lengths, repetition, presence, frequency
             raise SpeechAmdError("bias_ids and bias_values must have the same shape and strides")
     if mask is not None:
         words = (V + 31) // 32
-        if not torch.is_tensor(mask) or mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] < 1 or mask.shape[1] < words:
+        if not torch.is_tensor(mask) or mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] < min(rows, 1) or mask.shape[1] < words:
             raise SpeechAmdError("mask must be a (states, >= %d) int32 tensor (see pack_mask)" % words)
         if mask.device != dev or (mask.stride(1) != 1 and mask.shape[1] > 1):
             raise SpeechAmdError("mask must be on %s with a last stride of 1" % dev)

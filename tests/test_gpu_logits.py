@@ -216,6 +216,16 @@ def test_constrain_refuses_on_the_gpu():
     assert L().constrain(x[:0]).shape == (0, 40) and L().pick(x[:0])[0].shape == (0,)
 
 
+def test_a_batch_without_requests():
+    x = torch.zeros(0, 40).cuda()
+    none = torch.zeros(0, 5, dtype=torch.int64).cuda()
+    kw = dict(history=none, lengths=torch.zeros(0, dtype=torch.int32).cuda(), frequency=0.5, bias_ids=none, bias_values=torch.zeros(0, 5).cuda(),
+              mask=torch.zeros(0, 2, dtype=torch.int32).cuda())
+    assert L().constrain(x, **kw).shape == (0, 40)
+    tokens, logp = L().pick(x, **kw)
+    assert tokens.shape == logp.shape == (0,)
+
+
 # ---- top_logits ----------------------------------------------------------------------------------------------------------
 def check_top(x, k, temperature=1.0, got=None):
     values, ids, rest = L().top_logits(x.cuda(), k, temperature) if got is None else got

@@ -137,6 +137,21 @@ def test_the_c_entries_refuse_before_they_launch():
     assert lib.sa_logits_constrain(P, 8, 0, P, 8, 1 << 24, 8, ref, None) == bad
 
 
+def test_a_batch_without_requests_is_no_error():
+    """Empty tensors have no address: with no row there is nothing to read, whatever lists and masks come along."""
+    none = torch.zeros(0, 5, dtype=torch.int64)
+    i32 = torch.zeros(0, dtype=torch.int32)
+    words = L.pack_mask(torch.zeros(0, 40, dtype=torch.bool))
+    assert words.shape == (0, 2) and words.dtype == torch.int32
+    lib = _lib.lib()
+    for kw in (dict(history=none), dict(history=none, lengths=i32, repetition=torch.zeros(0), presence=0.5),
+               dict(bias_ids=none, bias_values=torch.zeros(0, 5)), dict(mask=words), dict(mask=words, states=i32),
+               dict(mask=torch.zeros(3, 2, dtype=torch.int32), states=i32)):
+        c = ctypes.byref(_check(rows=0, **kw))
+        assert lib.sa_logits_constrain(None, 40, 0, None, 40, 0, 40, c, None) == 0, list(kw)
+        assert lib.sa_logits_pick(None, 40, 0, 0, 40, c, None, None, None, 0, None) == 0, list(kw)
+
+
 def test_the_constrained_decode_refuses_before_it_launches():
     lib = _lib.lib()
     P, bad = 1 << 12, 2
