@@ -641,18 +641,29 @@ class Seq2Seq(Model):
 
     def top_logits(self, batch, k, temperature=1.0):
         """What this model, as a teacher, leaves of a batch for distill_loss: (values (B, U-1, k), ids (B, U-1, k), rest (B, U-1)),
-        the k largest logits of every output token and the log-sum-exp of the others (speech_amd.logits.top_logits)."""
+        the k largest logits of every output token and the log-sum-exp of the others (speech_amd.logits.top_logits).  A teacher
+        reads the labels it is given, without dropout: in training mode, too, which is as it was afterwards."""
         def run():
             with torch.no_grad():
                 out = _logits.top_logits(self(batch), k, temperature)
             torch.cuda.current_stream().synchronize()
             return out
-        return self._healthy(run)
+        training, sampling = [m for m in self.modules() if m.training], self.scheduled_sampling
+        self.scheduled_sampling = False
+        if training:
+            self.eval()
+        try:
+            return self._healthy(run)
+        finally:
+            self.scheduled_sampling = sampling
+            for m in training:
+                m.training = True
 
     def distill_loss(self, batch, values, ids, rest=None, weights=None, temperature=1.0, alpha=1.0):
         """The loss of this model, as a student, on a teacher's top logits: alpha T^2 KL + (1 - alpha) cross-entropy
         (speech_amd.logits.DistillLoss), summed over the tokens and divided by the batch size like loss() -- which it is at
-        alpha = 0.  `weights` (B, U-1) leaves padded tokens out (0); the reference scores them."""
+        alpha = 0.  `weights` (B, U-1) leaves padded tokens out (0); the reference scores them.  Under scheduled sampling the
+        student's rows follow what it was fed, like loss()'s."""
         x, y = self._collate_staged(*batch)
         if self.is_cuda:
             x = self._to_device(x)

@@ -202,6 +202,30 @@ def test_distillation_of_one_model_into_another(flatten):
     assert max(float(v.abs().max()) for v in grads(loss).values()) < 1e-3
 
 
+def test_a_teacher_in_training_mode_reads_the_labels():
+    """Dropout and scheduled sampling are the model's own training: the rows it teaches belong to the labels, and both are on again
+    afterwards, also when the call fails."""
+    from speech_amd._lib import SpeechAmdError
+    from speech_amd.models import Seq2Seq
+    cfg = {"dropout": 0.5, "encoder": CFG["encoder"], "decoder": dict(CFG["decoder"], sample_prob=0.5)}
+    torch.manual_seed(10)
+    m = Seq2Seq(40, VOCAB, cfg).cuda()
+    b = batch(6)
+    m.set_eval()
+    want = m.top_logits(b, 5, 2.0)
+    assert not m.training and not m.scheduled_sampling and m.volatile
+    m.set_train()
+    m.attend.eval()
+    for _ in range(3):
+        got = m.top_logits(b, 5, 2.0)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        assert m.training and m.scheduled_sampling and not m.volatile
+        assert not m.attend.training and not m.attend.conv.training and m.dec_rnn.training
+    with pytest.raises(SpeechAmdError):
+        m.top_logits(b, K + 1)
+    assert m.training and m.scheduled_sampling
+
+
 def test_teach_train_and_answer():
     """One small run of all of it: a few steps on a teacher's top logits, then answers under a grammar and penalties."""
     from speech_amd import ops
