@@ -123,6 +123,21 @@ def test_constrained_answers_obey_the_grammar_and_end_where_nothing_is_left():
     assert m.infer(batch(9), max_len=20, constraints=dict(mask=nothing)) == [[START, END]] * 5
 
 
+def test_constrained_infer_never_answers_nan():
+    """A token whose constrained logit is NaN is passed over, like one that is banned; with nothing else left the request ends."""
+    m = build(4)
+    m.set_eval()
+    g = torch.Generator().manual_seed(12)
+    ids = torch.stack([torch.randperm(K, generator=g)[:5] for _ in range(5)]).cuda()
+    b = batch(3)
+    def answers(value):
+        return m.infer(b, max_len=12, constraints=dict(bias_ids=ids, bias_values=torch.full((5, 5), value).cuda()))
+    assert answers(math.nan) == answers(-math.inf)
+    every = torch.arange(K).repeat(5, 1).cuda()
+    nan = torch.full((5, K), math.nan).cuda()
+    assert m.infer(b, max_len=12, constraints=dict(bias_ids=every, bias_values=nan)) == [[START, END]] * 5
+
+
 def test_constrained_infer_refuses():
     from speech_amd._lib import SpeechAmdError
     m = build(5)
