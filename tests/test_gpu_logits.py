@@ -287,6 +287,38 @@ def test_top_logits_of_rows_that_are_not_ordinary(V, times, k):
         check_top(y, k, 1.0, got=[t[0] for t in many])
 
 
+@pytest.mark.parametrize("V,times", [(29, 1), (300, 1), (5000, 1), (40000, 1), (300, 86), (1000, 86), (9000, 22), (30000, 22)])
+@pytest.mark.parametrize("k", [1, 20, 128])
+def test_the_rest_of_rows_that_are_not_ordinary(V, times, k):
+    """Like the rows above, each held to the tolerance of its own range: where all of the top lies in one stretch or at one step, many
+    ties, all equal, a second stretch far below, a slope."""
+    k = min(k, V)
+    g = gen(V * k + 1)
+    x = torch.randn(12, V, generator=g)
+    x[0] = 1.5
+    x[1] = torch.arange(V).float() * (20.0 / V)
+    x[2] = -torch.arange(V).float() * (20.0 / V)
+    x[3, ::2] = -math.inf
+    x[4, [0, V - 1]] = math.inf
+    x[5] = torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0)
+    x[6, :min(V, 400)] += 50
+    x[7, 4::max(1, V // 37)] += 50
+    x[8] = torch.randint(0, 3, (V,), generator=g).float()
+    x[9] = -x[9].abs() - 100
+    x[10, V // 2:] -= 30
+    x[11] *= 5
+    for dtype in TYPES:
+        y = x.to(dtype)
+        many = L().top_logits(y.cuda().repeat(times, 1), k)
+        many = [t.view(times, 12, *t.shape[1:])[0] for t in many]
+        for row in range(12):
+            check_top(y[row:row + 1], k, 1.0, got=[t[row:row + 1] for t in many])
+    low = torch.full((3, V), torch.finfo(torch.float32).min)   # the type's lowest value is a number: rest = it + log(V - k) = it
+    rest = L().top_logits(low.cuda(), k)[2]
+    want = low[0, 0] if V > k else torch.tensor(-math.inf)
+    assert bool((rest.cpu() == want).all())
+
+
 @pytest.mark.parametrize("V,times", [(129, 1), (700, 1), (1000, 64), (9000, 16), (30000, 16), (40000, 1), (200001, 1)])
 @pytest.mark.parametrize("k", [5, 128])
 def test_top_logits_of_masked_rows(V, times, k):
@@ -783,6 +815,40 @@ def test_captured_graphs():
         for i in (0, 1):
             for a, b in zip(outs[i], want[i]):
                 assert torch.equal(a.float().nan_to_num(nan=1e30), b.float().nan_to_num(nan=1e30)), (trip, i)
+
+
+@pytest.mark.parametrize("V,dtype", [(140000, torch.float32), (300007, torch.float32), (280001, torch.bfloat16)])
+def test_captured_graphs_of_rows_beyond_the_registers(V, dtype):
+    """Rows that the loss keeps in LDS, more than 48 KB of it: the kernel's limit is raised inside the capture too."""
+    g = gen(V)
+    n = 3
+    inputs = [rows_like(g, n, V, dtype).cuda() for _ in range(3)]
+    _, sk = student(g, n, V, dtype, 16, 2.0)
+    sk = cuda(sk)
+    static = inputs[0].clone().requires_grad_(True)
+
+    def step(x):
+        x.grad = None
+        loss = L().DistillLoss(2.0, 0.5, denom=n / 256.0)(x, **sk)
+        loss.backward()
+        return [loss.detach(), x.grad]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    static.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for trip in range(4):
+        with torch.no_grad():
+            static.copy_(inputs[trip % 3])
+        graph.replay()
+        want = step(inputs[trip % 3].clone().requires_grad_(True))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), trip
 
 
 def test_same_bits_on_every_run():
