@@ -4,10 +4,12 @@ speech/utils/io.py:15-19: torch.save of the WHOLE module + a pickled Preprocesso
 speech.load() of this repo reads the reference's on-disk format.  Build container only:
     python oracle/gen_ref_checkpoint.py
 Outputs tests/golden/ref_ckpt/<name>_model, <name>_preproc.pyc (the reference's file naming with tag = <name>) and
-tests/golden/ref_ckpt.npz (a seeded input batch and the reference's outputs for it).
+tests/golden/ref_ckpt.npz (a seeded input batch and the reference's outputs for it); preproc.pickle beside them is a copy of one
+of the (equal) <name>_preproc.pyc, for places that *.pyc files do not reach (tests/conftest.py).
 Nothing is copied from the reference; it is only executed (import recipe: oracle/gen_golden.py).
 """
 import os
+import shutil
 import sys
 
 import numpy as np
@@ -62,6 +64,7 @@ def main():
         arrays[name + ".enc"] = enc.numpy()
         arrays[name + ".keys"] = np.array(sorted(model.state_dict().keys()))
         print(name, "saved;", type(model).__module__, "enc", tuple(enc.shape))
+    shutil.copyfile(os.path.join(OUT, "ctc_preproc.pyc"), os.path.join(OUT, "preproc.pickle"))
     arrays["preproc.mean"] = np.asarray(preproc.mean)
     arrays["preproc.vocab"] = np.array(preproc.vocab_size)
     np.savez_compressed(os.path.join(OUT, "..", "ref_ckpt.npz"), **arrays)

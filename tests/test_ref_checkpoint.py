@@ -75,3 +75,17 @@ def test_loaded_reference_checkpoint_encodes_like_the_reference(golden_dir, name
     with torch.no_grad():
         enc = model.encode(torch.from_numpy(z[name + ".x"]).cuda())
     np.testing.assert_allclose(enc.cpu().numpy(), z[name + ".enc"], rtol=2e-4, atol=2e-5)
+
+
+def test_preprocessors_that_did_not_travel_come_back(golden_dir, tmp_path):
+    import shutil
+    from .conftest import restore_preprocessors
+    here = os.path.join(golden_dir, "ref_ckpt")
+    shutil.copyfile(os.path.join(here, "preproc.pickle"), str(tmp_path / "preproc.pickle"))
+    (tmp_path / "ctc_preproc.pyc").write_bytes(b"mine")          # what is there stays
+    restore_preprocessors(str(tmp_path))
+    assert (tmp_path / "ctc_preproc.pyc").read_bytes() == b"mine"
+    for name in set(NAMES) - {"ctc"}:
+        with open(os.path.join(here, name + "_preproc.pyc"), "rb") as fid:
+            assert (tmp_path / (name + "_preproc.pyc")).read_bytes() == fid.read()
+    assert len(list(tmp_path.iterdir())) == 1 + len(NAMES)
