@@ -38,11 +38,10 @@ __device__ __forceinline__ float dis_base(float m) { return m == -INFINITY ? 0.0
 // REST: the rest is a class, and the list is taken out of the sums.  The sum at temperature 1 beside the one at T, HARD: 0 not wanted
 // or the same; 1 by its own exponential; 2, 4 as that power of the one at T = 2, 4.
 // MORE: rows longer than the registers hold.
-template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST, int HARD>
+template <typename T, int NT, int NV, bool MORE, bool REST, int HARD>
 __global__ __launch_bounds__(NT) void distill_kernel(const T* __restrict__ x, T* dx, SaRows at, int V, int stash, DisArgs A) {
     constexpr int VEC = SaVec<T>::N, NW = NT / 64;
-    constexpr bool TWO = HARD != 0;
-    static_assert(!KEEP || HARD != 1, "only one exponential of an element is kept");
+    constexpr bool TWO = HARD != 0, KEEP = HARD != 1;  // (only one exponential of an element is kept)
     extern __shared__ uint4 held[];                // `stash` vectors a thread, and behind them
     unsigned* bitmap = (unsigned*)(held + stash * NT);  // a bit per element of the row's vectors: the token is in the list
     __shared__ DisSum waves[NW];
@@ -352,7 +351,7 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float* __restri
     }
 }
 
-template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST, int HARD>
+template <typename T, int NT, int NV, bool MORE, bool REST, int HARD>
 bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
     // rows beyond the registers: as many vectors as 152 KB of LDS hold beside the bitmap
     const size_t bits = (size_t)((V + 2 * SaVec<T>::N + 31) / 32) * 4;
@@ -360,7 +359,7 @@ bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const 
     int stash = MORE && more > 0 ? (int)((152 * 1024 - bits) / (16 * NT)) : 0;
     if (stash * NT > more) stash = more > 0 ? (more + NT - 1) / NT : 0;
     const size_t smem = bits + (size_t)stash * NT * 16;
-    constexpr auto kernel = distill_kernel<T, NT, NV, KEEP && HARD != 1, MORE, REST, HARD>;
+    constexpr auto kernel = distill_kernel<T, NT, NV, MORE, REST, HARD>;
     if (smem > 48 * 1024 &&
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
         return false;
@@ -368,18 +367,18 @@ bool dis_run(const void* x, void* dx, const SaRows& at, long rows, int V, const 
     return true;
 }
 
-template <typename T, int NT, int NV, bool KEEP, bool MORE, bool REST>
+template <typename T, int NT, int NV, bool MORE, bool REST>
 bool dis_hard(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    if (A.alpha == 1.0f || !A.targets || A.temperature == 1.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 0>(x, dx, at, rows, V, A, stream);
-    if (A.temperature == 2.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 2>(x, dx, at, rows, V, A, stream);
-    if (A.temperature == 4.0f) return dis_run<T, NT, NV, KEEP, MORE, REST, 4>(x, dx, at, rows, V, A, stream);
-    return dis_run<T, NT, NV, KEEP, MORE, REST, 1>(x, dx, at, rows, V, A, stream);
+    if (A.alpha == 1.0f || !A.targets || A.temperature == 1.0f) return dis_run<T, NT, NV, MORE, REST, 0>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 2.0f) return dis_run<T, NT, NV, MORE, REST, 2>(x, dx, at, rows, V, A, stream);
+    if (A.temperature == 4.0f) return dis_run<T, NT, NV, MORE, REST, 4>(x, dx, at, rows, V, A, stream);
+    return dis_run<T, NT, NV, MORE, REST, 1>(x, dx, at, rows, V, A, stream);
 }
 
-template <typename T, int NT, int NV, bool KEEP, bool MORE = false>
+template <typename T, int NT, int NV, bool MORE = false>
 bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
-    return A.rest ? dis_hard<T, NT, NV, KEEP, MORE, true>(x, dx, at, rows, V, A, stream)
-                  : dis_hard<T, NT, NV, KEEP, MORE, false>(x, dx, at, rows, V, A, stream);
+    return A.rest ? dis_hard<T, NT, NV, MORE, true>(x, dx, at, rows, V, A, stream)
+                  : dis_hard<T, NT, NV, MORE, false>(x, dx, at, rows, V, A, stream);
 }
 
 // The smallest workgroup whose registers hold a row, 64 exponentials a thread at most: up to 128 registers a thread, so that the
@@ -388,20 +387,27 @@ bool dis_pick(const void* x, void* dx, const SaRows& at, long rows, int V, const
 // keeps what it can in LDS: 1024 threads, 256 KB in registers and 128 KB in LDS (2048 x 131072 f32: 440 us; without LDS 534, two
 // smaller workgroups on a CU 580 - 615, all of them bound by what is read twice).  A short row is one wave's, without any exchange
 // (16000 x 1000 f32: 31 us against 54 with 256 threads, 8000 x 2000 bf16: 24.5 against 41.6).
-int dis_threads(int vectors, int vec) {
-    return vectors <= 64 * 4 ? 64 : vectors <= 256 * 4 ? 256 : vectors <= 512 * 64 / vec ? 512 : 1024;
+struct DisForm { int nt, nv; bool more; };  // threads, vectors a thread holds in registers, rows beyond that
+DisForm dis_form(int V, int vec) {
+    const int vectors = (V + 2 * vec - 2) / vec;  // of the longest row, with its lead
+    if (vectors <= 64 * 2) return {64, 2, false};
+    if (vectors <= 64 * 4) return {64, 4, false};
+    if (vectors <= 256 * 4) return {256, 4, false};
+    if (vectors <= 512 * 32 / vec) return {512, 32 / vec, false};
+    if (vectors <= 512 * 64 / vec) return {512, 64 / vec, false};
+    return {1024, 64 / vec, vectors > 1024 * 64 / vec};
 }
 template <typename T>
 bool dis_launch(const void* x, void* dx, const SaRows& at, long rows, int V, const DisArgs& A, hipStream_t stream) {
     constexpr int VEC = SaVec<T>::N;
-    const int vectors = (V + 2 * VEC - 2) / VEC;
-    if (vectors <= 64 * 2) return dis_pick<T, 64, 2, true>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 64 * 4) return dis_pick<T, 64, 4, true>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 256 * 4) return dis_pick<T, 256, 4, true>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 512 * 32 / VEC) return dis_pick<T, 512, 32 / VEC, true>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 512 * 64 / VEC) return dis_pick<T, 512, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
-    if (vectors <= 1024 * 64 / VEC) return dis_pick<T, 1024, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
-    return dis_pick<T, 1024, 64 / VEC, true, true>(x, dx, at, rows, V, A, stream);
+    const DisForm f = dis_form(V, VEC);
+    if (f.nt == 64 && f.nv == 2) return dis_pick<T, 64, 2>(x, dx, at, rows, V, A, stream);
+    if (f.nt == 64) return dis_pick<T, 64, 4>(x, dx, at, rows, V, A, stream);
+    if (f.nt == 256) return dis_pick<T, 256, 4>(x, dx, at, rows, V, A, stream);
+    if (f.nt == 512 && f.nv == 32 / VEC) return dis_pick<T, 512, 32 / VEC>(x, dx, at, rows, V, A, stream);
+    if (f.nt == 512) return dis_pick<T, 512, 64 / VEC>(x, dx, at, rows, V, A, stream);
+    if (!f.more) return dis_pick<T, 1024, 64 / VEC>(x, dx, at, rows, V, A, stream);
+    return dis_pick<T, 1024, 64 / VEC, true>(x, dx, at, rows, V, A, stream);
 }
 
 }  // namespace
@@ -416,8 +422,7 @@ extern "C" ctcStatus_t sa_distill_loss(const void* x, void* dx, long ld_outer, l
         !sa_temperature_ok(temperature) || !(alpha >= 0.f && alpha <= 1.f) || (rows > 0 && !loss && !dx) ||
         (loss && !loss_rows && rows > 0))
         return CTC_STATUS_INVALID_VALUE;
-    const int vec = dtype == SA_F32 ? 4 : 8;
-    if (!sa_threads_ok(rows, dis_threads((V + 2 * vec - 2) / vec, vec))) return CTC_STATUS_INVALID_VALUE;
+    if (!sa_threads_ok(rows, dis_form(V, dtype == SA_F32 ? 4 : 8).nt)) return CTC_STATUS_INVALID_VALUE;
     hipStream_t stream = (hipStream_t)stream_;
     if (rows > 0) {
         if (!x || !values || !ids) return CTC_STATUS_INVALID_VALUE;
