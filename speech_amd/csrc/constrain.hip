@@ -290,8 +290,10 @@ void con_launch(const void* x, long ldx, void* y, long ldy, int rows, int V, con
         if constexpr (!PICK) CON_LAUNCH(512, 16 / SaVec<T>::N);
     } else if (p.nv == 1) CON_LAUNCH(256, 1);
     else if (p.nv == 2) CON_LAUNCH(256, 2);
-    else if (p.nv == 4) CON_LAUNCH(256, 4);
-    else if constexpr (PICK && sizeof(T) == 4) CON_LAUNCH(256, 8);
+    else if constexpr (PICK || sizeof(T) == 4) {  // (con_plan's most: 16 / VEC, twice that for pick)
+        if (p.nv == 4) CON_LAUNCH(256, 4);
+        else if constexpr (PICK && sizeof(T) == 4) CON_LAUNCH(256, 8);
+    }
 #undef CON_LAUNCH
 }
 

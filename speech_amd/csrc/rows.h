@@ -28,7 +28,6 @@ struct SaRows {
     }
 };
 
-static inline size_t sa_type_bytes(int dtype) { return dtype == SA_F32 ? 4 : 2; }
 static inline bool sa_temperature_ok(float t) { return t >= 0.99e-6f && t <= 1.01e6f; }  // T^2 and x / T stay in 32 bits
 static inline bool sa_rows_ok(int dtype, int V) { return dtype >= SA_F32 && dtype <= SA_F16 && V >= 1 && V <= SA_VOCAB_MAX; }
 // a launch holds fewer than 2^32 threads (its last workgroup filled up)
