@@ -607,7 +607,9 @@ ctcStatus_t sa_logits_pick(const void* x, long ldx, int dtype, int rows, int V, 
  * states are not read.  penalties != 0: the history of request b is its row of d_tokens so far (the start token is no class).
  * d_states (rows) int, with a mask: the request's mask row, moved on to d_next_states[state * K + token] ((n_states, K) int, or
  * NULL: it stays) after every token; a state outside the mask is unmasked from then on.  A request that has no token left emits
- * end_tok; a NaN logit is passed over as in the plain decode (sa_logits_pick takes it for the largest).  max_len < SA_LIST_MAX; workspace: sa_s2s_greedy_workspace_bytes. */
+ * end_tok; a NaN logit is passed over as in the plain decode (sa_logits_pick takes it for the largest).  As there, a request that has
+ * ended goes on until all of them emit end_tok in one step, under its constraints.  max_len < SA_LIST_MAX; workspace:
+ * sa_s2s_greedy_workspace_bytes. */
 ctcStatus_t sa_s2s_greedy_decode_constrained(const float* eh, const float* const* params, int B, int T, int H, int E, int KS,
                                              int K, float scale, int end_tok, int max_len, int check_every,
                                              const saConstraints* c, int penalties, int* d_states, const int* d_next_states,

@@ -9,7 +9,9 @@
 // A workgroup per row.  The row is read once, as 16-byte vectors, into registers (what is beyond NT * NV vectors is read a second
 // time); each thread sums relative to its own maximum, the waves' results are joined in one exchange through LDS, and the
 // gradient is formed from the registers: from the exponentials themselves where they fit (KEEP), one or two multiplications an
-// element, else from the logits again.  At T = 2 and T = 4 the second sum takes exp(x - m) as a power of exp((x - m) / T).
+// element, else from the logits again.  At T = 2 and T = 4 the second sum takes exp(x - m) as a power of exp((x - m) / T): 4096 x 32000
+// bf16 115 us a call where exponentials of its own, taken again for the gradient, cost 155, 2048 x 131072 f32 440 against 481, 1000 x
+// 50021 f16 71 against 79; that is what other temperatures with hard targets cost (T = 3: 153, 480, 79).
 // Listed tokens are marked in a bitmap in LDS and taken out of the sums where the rest is a class of its own; their gradients
 // replace what the row-wide formula wrote.  The teacher's side of a row is k <= 128
 // numbers: the first wave does it, two to a lane, while the others sum.

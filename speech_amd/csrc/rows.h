@@ -76,7 +76,7 @@ __device__ __forceinline__ unsigned long long sa_rank_key(float x, int i) {
 // ---- a row as vectors of 16 bytes ------------------------------------------------------------------------------------------
 // Rows start anywhere (odd V, views): vector q of a row covers its elements [q VEC - lead, q VEC - lead + VEC), where `lead` is how
 // many elements the row starts behind a 16-byte boundary.  Every whole vector is then one aligned 16-byte access and only a row's
-// first and last vector can be partial; those go element by element, so nothing outside the row is touched.
+// first and last vector can be partial: those are accessed by elements of the row alone, so nothing outside it is touched.
 template <typename T> struct SaVec { static constexpr int N = 16 / (int)sizeof(T); };
 template <typename T> __device__ __forceinline__ unsigned sa_fill_word();  // -inf in every element
 template <> __device__ __forceinline__ unsigned sa_fill_word<float>() { return 0xff800000u; }
@@ -145,8 +145,9 @@ template <typename T> __device__ __forceinline__ void sa_store_vec(T* row, int v
 
 // The vector whose first element is v0 (a multiple of VEC minus lead); -inf outside [0, V).  A row's first and last vector: all their
 // elements at once, those outside taken from the row's ends and dropped -- one wait, where one element after the other costs rows of
-// odd lengths 10 - 20 % (8000 x 5001 bf16: top logits 48 -> 42 us, constrain 52 -> 43, distillation 54 -> 48).  TIGHT: one after the
-// other after all, for kernels without the registers (top logits, 4096 x 32000 bf16: 71 us against 78).
+// odd lengths 10 - 20 % (8000 x 5001 bf16: top logits 48 -> 42 us, constrain 52 -> 43, distillation 54 -> 48).  The registers it takes
+// cost rows without partial vectors something (pick, 4096 x 32000 bf16: 99 -> 108 us).  TIGHT: one after the other, for kernels that
+// have none to spare (top logits, bf16: 83 us a launch against 86 at 4096 x 32000, but 94 against 86 at 4096 x 32001).
 template <typename T, bool TIGHT = false> __device__ __forceinline__ uint4 sa_load_vec(const T* row, int v0, int V) {
     if (v0 >= 0 && v0 + SaVec<T>::N <= V) return *reinterpret_cast<const uint4*>(row + v0);
     constexpr int N = SaVec<T>::N, BITS = 8 * (int)sizeof(T);

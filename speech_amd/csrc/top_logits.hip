@@ -9,7 +9,7 @@
 // than k of thousands in ordinary rows, and everything below it goes straight into the log-sum-exp, relative to the bound.  The
 // candidates are ranked against each other in LDS.  Where that does not hold -- rows that are masked or constant but for a few
 // elements, NaN, a rest that vanishes beside the bound -- the workgroup looks for a better cut by halving, at a pass over the row in
-// the caches for each step (4096 x 32000 bf16, k = 64, constant rows: 240 us against 78 for ordinary ones).
+// the caches for each step (4096 x 32000 bf16, k = 64, constant rows: 240 us a call against 80 for ordinary ones).
 #include "rows.h"
 
 namespace {
@@ -146,8 +146,9 @@ __device__ __forceinline__ void top_write_rest(float m, float s, float temperatu
 // A segment of a row: `per` <= NT * NV vectors; nseg == 1: the whole row, and the result.  (The segments of a row are of equal
 // length: a short last one would have fewer than k threads with anything, no bound, and take the exact way.)
 // It is a chain of short phases, and what hides one is another workgroup's: registers for six waves a SIMD (4096 x 32000 bf16, k = 64:
-// 81 us on most boxes, where the bytes alone would take 52; registers for eight waves, with spills, 128; unbounded 132).  Without the
-// exponentials it takes 75, without the ranking 76, with a bound known beforehand 58: no one phase bounds it.
+// 80 us a call, 82 - 88 a launch under the profiler, where the bytes alone would take 52).  Compared in runs that put it at 81:
+// registers for eight waves, with spills, 128; unbounded 132; without the exponentials 75, without the ranking 76, with a bound known
+// beforehand 58: no one phase bounds it.
 template <typename T, int NT, int NV>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(6))) void top_segment_kernel(
     const T* __restrict__ x, SaRows at, int V, int k, int cap, float temperature, int nseg, int per, TopOut out,
@@ -509,8 +510,8 @@ __global__ __launch_bounds__(256) void top_short_kernel(const T* __restrict__ x,
     if (lane == 0) top_write_rest(m, s, temperature, out.rest + row);
 }
 
-// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16: 81 us
-// whole, 90 + 23 in two segments and a merge), and a wave takes a row of up to 1000 (2000 of two bytes) when every SIMD gets one:
+// Rows that a workgroup's registers hold are not split when there are enough of them to fill the device (4096 x 32000 bf16, in the same
+// runs: 81 us whole, 90 + 23 in two segments and a merge), and a wave takes a row of up to 1000 (2000 of two bytes) when every SIMD gets one:
 // no exchange between waves (16000 x 1000 f32, k = 8: 25 us against 58 with 256 threads; 16000 x 1000 bf16, k = 64: 40 against 98; at twice
 // the length 33 against 36 and 32 against 30).  Others are split into segments of 256 threads, shorter ones where there are few
 // rows, as long as one workgroup can hold what the segments leave.

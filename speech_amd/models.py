@@ -721,7 +721,8 @@ class Seq2Seq(Model):
         """seq2seq.py:160-178: greedy decode from the start tokens (no beam search).
         constraints: penalties for repeated tokens, biases and a grammar that every token is held to, a dict of
         speech_amd.logits.decoding_constraints' arguments (requests = utterances, V = vocab_size - 1 classes); an utterance
-        that has no token left emits the end token."""
+        that has no token left emits the end token.  As without them, an utterance that has ended goes on until all emit the
+        end token in one step: an answer is what stands before its first end token (which penalties lower like any other)."""
         x, y = self._collate_staged(*batch)
         end_tok = int(y[0, -1])
 
