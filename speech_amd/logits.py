@@ -357,11 +357,11 @@ class DistillLoss(torch.nn.Module):
             raise SpeechAmdError("denom must be within 1e-30 .. 1e30, got %r" % denom)
 
     def forward(self, logits, values, ids, rest=None, targets=None, weights=None):
-        if not torch.is_tensor(values) or not 1 <= values.shape[-1] <= TOP_MAX:
+        if not torch.is_tensor(values) or values.dim() < 1 or not 1 <= values.shape[-1] <= TOP_MAX:
             raise SpeechAmdError("values must be a (..., k) tensor with 1 <= k <= %d" % TOP_MAX)
         if self.alpha < 1.0 and targets is None:
             raise SpeechAmdError("alpha < 1 mixes in hard targets: targets are needed")
-        if not torch.is_tensor(logits):
-            raise SpeechAmdError("logits must be a tensor")
+        if not torch.is_tensor(logits) or logits.dim() < 1:
+            raise SpeechAmdError("logits must be a (..., V) tensor")
         denom = float(self.denom) if self.denom else float(max(1, logits.numel() // max(1, logits.shape[-1])))
         return DistillFunction.apply(logits, values, ids, rest, targets, weights, self.temperature, self.alpha, 1.0 / denom)

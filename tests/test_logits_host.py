@@ -89,6 +89,16 @@ def test_parameters_of_the_loss_are_checked():
             L._temperature(t)
 
 
+def test_numbers_in_place_of_rows_are_refused():
+    x, v, i = torch.zeros(2, 8), torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int64)
+    for logits, values in ((x, v[0, 0]), (x[0, 0], v), (x, 1.0), (1.0, v), (x, None)):
+        with pytest.raises(SpeechAmdError):
+            L.DistillLoss()(logits, values, i)
+    for call in (L.constrain, L.pick, lambda t: L.top_logits(t, 1)):
+        with pytest.raises(SpeechAmdError):
+            call(x[0, 0])
+
+
 def test_the_c_entries_refuse_before_they_launch():
     lib = _lib.lib()
     c = _lib.saConstraints()
